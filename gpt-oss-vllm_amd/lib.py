@@ -32,7 +32,8 @@ EXPORTS = (
     "m355_moe_nf4_forward_routed", "m355_attn_prefill", "m355_moe_combine_add_rmsnorm", "m355_init",
     "m355_moe_nf4_forward_static", "m355_router_topk_ep_pack", "m355_moe_nf4_forward_ep_rows", "m355_ep_reduce_add_rmsnorm",
     "m355_qkv_rope_kv_write", "m355_moe_nf4_forward_logits", "m355_norm_qkv_rope_kv_write",
-    "m355_time_next_launch", "m355_timed_launch_us",
+    "m355_time_next_launch", "m355_timed_launch_us", "m355_shared_prefix_attn", "m355_shared_prefix_attn_workspace_bytes",
+    "m355_paged_attn_decode_scored", "m355_paged_attn_decode_scored_workspace_bytes", "m355_kv_evict",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -121,6 +122,16 @@ def load() -> ctypes.CDLL:
     L.m355_time_next_launch.restype = i32
     L.m355_timed_launch_us.argtypes = [ctypes.POINTER(ctypes.c_float)]
     L.m355_timed_launch_us.restype = i32
+    L.m355_shared_prefix_attn.argtypes = [vp] * 6 + [i32] * 10 + [i64, i32, i32, i64, i64, f32, vp, i32, vp, sz, vp, vp]
+    L.m355_shared_prefix_attn.restype = i32
+    L.m355_shared_prefix_attn_workspace_bytes.argtypes = [i32] * 8
+    L.m355_shared_prefix_attn_workspace_bytes.restype = sz
+    L.m355_paged_attn_decode_scored.argtypes = [vp] * 6 + [i32] * 8 + [i64, i32, i32, i64, i64, f32, vp, i32, vp, sz, vp, vp]
+    L.m355_paged_attn_decode_scored.restype = i32
+    L.m355_paged_attn_decode_scored_workspace_bytes.argtypes = [i32] * 6
+    L.m355_paged_attn_decode_scored_workspace_bytes.restype = sz
+    L.m355_kv_evict.argtypes = [vp] * 6 + [i32] * 7 + [i64, i32, i32, i32, i32, vp, vp, vp]
+    L.m355_kv_evict.restype = i32
     for fn in ("m355_ep_pack", "m355_ep_unpack", "m355_ep_reduce", "m355_nf4_dequant", "m355_repack_nf4", "m355_router_topk", "m355_topk_softmax",
                "m355_moe_nf4_forward", "m355_paged_attn_decode", "m355_add_rmsnorm", "m355_rope_kv_write"):
         getattr(L, fn).restype = i32
@@ -759,3 +770,168 @@ def attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: 
                                     None if sinks is None else _dev(sinks, torch.float16, "sinks"), int(window),
                                     _dev(out, torch.float16, "out"), _stream()), "m355_attn_prefill")
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# long contexts: a shared prefix, accumulated attention weights, eviction
+# ---------------------------------------------------------------------------------------------
+_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}   # M355_DTYPE_F16, M355_DTYPE_BF16
+
+
+def _one_device(**tensors) -> None:
+    """All tensors on the GPU that is current: a launch goes to the current device's current stream."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise Mi355LibraryError(f"{name} must be a GPU tensor; this path has no CPU implementation")
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype):
+    """(pointer, token stride) of a [tokens][heads][D] tensor whose tokens may be strided."""
+    T, heads, D = t.shape
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if (D > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != D):
+        raise ValueError(f"{name} must have contiguous heads")
+    return t.data_ptr(), t.stride(0) if T > 1 else heads * D
+
+
+def _paged_cache(kcache: torch.Tensor, vcache: torch.Tensor, dtype: torch.dtype) -> int:
+    """Page stride in elements of caches [blocks][block_size][Hkv][D]; pages may be strided (K and V of one page side by
+    side, say), a page itself is contiguous."""
+    if kcache.dim() != 4 or kcache.shape != vcache.shape:
+        raise ValueError("caches must be [blocks][block_size][Hkv][D], both alike")
+    if kcache.dtype != dtype or vcache.dtype != dtype:
+        raise TypeError(f"caches must be {dtype}, got {kcache.dtype} and {vcache.dtype}")
+    n, bs, hkv, d = kcache.shape
+    for name, t in (("kcache", kcache), ("vcache", vcache)):
+        if (d > 1 and t.stride(3) != 1) or (hkv > 1 and t.stride(2) != d) or (bs > 1 and t.stride(1) != hkv * d):
+            raise ValueError(f"{name}: a page must be contiguous")
+    if n > 1 and kcache.stride(0) != vcache.stride(0):
+        raise ValueError("caches must share their page stride")
+    return kcache.stride(0) if n > 1 else bs * hkv * d
+
+
+def shared_prefix_attn_workspace_bytes(T: int, B: int, max_q: int, Hq: int, Hkv: int, D: int, max_ctx: int, prefix_len: int) -> int:
+    return int(load().m355_shared_prefix_attn_workspace_bytes(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len))
+
+
+def shared_prefix_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, *,
+                       prefix_len: int, max_ctx: int, scale: float, seq_starts: Optional[torch.Tensor] = None, max_q: int = 1,
+                       sinks: Optional[torch.Tensor] = None, window: int = 0, workspace: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None):
+    """Attention of new tokens q [T][Hq][D] (fp16 or bf16; tokens may be strided) over a paged cache whose first prefix_len
+    tokens, read through row 0 of block_tables, all sequences share.  seq_starts int32 [B + 1] gives the sequences' tokens,
+    max_q the longest one's number; without it there is one token per sequence.  ctx_lens count the new tokens.
+    m355_shared_prefix_attn."""
+    _one_device(q=q, kcache=kcache, vcache=vcache, block_tables=block_tables, ctx_lens=ctx_lens, seq_starts=seq_starts, sinks=sinks,
+                workspace=workspace, out=out)
+    if q.dtype not in _DTYPE_CODES:
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    T, Hq, D = q.shape
+    B, max_blocks = block_tables.shape
+    nblocks, block_size, Hkv, Dc = kcache.shape
+    if Dc != D:
+        raise ValueError(f"q has heads of {D}, the cache of {Dc}")
+    if ctx_lens.numel() != B or (seq_starts is not None and seq_starts.numel() != B + 1):
+        raise ValueError(f"block_tables has {B} rows, ctx_lens {ctx_lens.numel()} entries"
+                         + ("" if seq_starts is None else f", seq_starts {seq_starts.numel()} (one more is needed)"))
+    if sinks is not None and sinks.numel() != Hq:
+        raise ValueError(f"sinks has {sinks.numel()} entries, expected one per query head ({Hq})")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, expected {tuple(q.shape)}")
+    stride = _paged_cache(kcache, vcache, q.dtype)
+    q_ptr, q_stride = _token_rows(q, "q", q.dtype)
+    o_ptr, o_stride = _token_rows(out, "out", q.dtype)
+    if workspace is None:
+        workspace = torch.empty(max(256, shared_prefix_attn_workspace_bytes(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len)), dtype=torch.uint8,
+                                device=q.device)
+    _check(load().m355_shared_prefix_attn(
+        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _dev(block_tables, torch.int32, "block_tables"), _dev(ctx_lens, torch.int32, "ctx_lens"),
+        None if seq_starts is None else _dev(seq_starts, torch.int32, "seq_starts"), T, B, int(max_q), Hq, Hkv, D, _DTYPE_CODES[q.dtype],
+        nblocks, block_size, max_blocks, stride, int(max_ctx), int(prefix_len), q_stride, o_stride, float(scale),
+        None if sinks is None else _dev(sinks, q.dtype, "sinks"), int(window), _dev(workspace, torch.uint8, "workspace"), workspace.numel(),
+        o_ptr, _stream()), "m355_shared_prefix_attn")
+    return out
+
+
+def paged_attn_decode_scored_workspace_bytes(B: int, Hq: int, Hkv: int, D: int, max_ctx: int, prefix_len: int = 0) -> int:
+    return int(load().m355_paged_attn_decode_scored_workspace_bytes(B, Hq, Hkv, D, max_ctx, prefix_len))
+
+
+def _page_scores(scores: torch.Tensor, kcache: torch.Tensor) -> int:
+    nblocks, block_size, Hkv, _ = kcache.shape
+    if tuple(scores.shape) != (nblocks, Hkv, block_size):
+        raise ValueError(f"scores is {tuple(scores.shape)}, expected {(nblocks, Hkv, block_size)}")
+    return _dev(scores, torch.float32, "scores")
+
+
+def paged_attn_decode_scored(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, scores: torch.Tensor, block_tables: torch.Tensor,
+                             ctx_lens: torch.Tensor, *, max_ctx: int, scale: float, prefix_len: int = 0,
+                             sinks: Optional[torch.Tensor] = None, window: int = 0, workspace: Optional[torch.Tensor] = None,
+                             out: Optional[torch.Tensor] = None):
+    """shared_prefix_attn with one token per sequence, which also adds the attention weight of every own token (positions
+    from prefix_len on), summed over a KV head's query heads, to scores [blocks][Hkv][block_size] fp32.  Zero a page's
+    scores when the page is handed out.  m355_paged_attn_decode_scored."""
+    _one_device(q=q, kcache=kcache, vcache=vcache, scores=scores, block_tables=block_tables, ctx_lens=ctx_lens, sinks=sinks,
+                workspace=workspace, out=out)
+    if q.dtype not in _DTYPE_CODES:
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    B, Hq, D = q.shape
+    nblocks, block_size, Hkv, Dc = kcache.shape
+    if Dc != D:
+        raise ValueError(f"q has heads of {D}, the cache of {Dc}")
+    if block_tables.shape[0] != B or ctx_lens.numel() != B:
+        raise ValueError(f"block_tables has {block_tables.shape[0]} rows, ctx_lens {ctx_lens.numel()} entries for {B} tokens")
+    if sinks is not None and sinks.numel() != Hq:
+        raise ValueError(f"sinks has {sinks.numel()} entries, expected one per query head ({Hq})")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, expected {tuple(q.shape)}")
+    stride = _paged_cache(kcache, vcache, q.dtype)
+    q_ptr, q_stride = _token_rows(q, "q", q.dtype)
+    o_ptr, o_stride = _token_rows(out, "out", q.dtype)
+    if workspace is None:
+        workspace = torch.empty(max(256, paged_attn_decode_scored_workspace_bytes(B, Hq, Hkv, D, max_ctx, prefix_len)), dtype=torch.uint8,
+                                device=q.device)
+    _check(load().m355_paged_attn_decode_scored(
+        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _dev(block_tables, torch.int32, "block_tables"),
+        _dev(ctx_lens, torch.int32, "ctx_lens"), B, Hq, Hkv, D, _DTYPE_CODES[q.dtype], nblocks, block_size, block_tables.shape[1], stride,
+        int(max_ctx), int(prefix_len), q_stride, o_stride, float(scale), None if sinks is None else _dev(sinks, q.dtype, "sinks"),
+        int(window), _dev(workspace, torch.uint8, "workspace"), workspace.numel(), o_ptr, _stream()), "m355_paged_attn_decode_scored")
+    return out
+
+
+def kv_evict(kcache: torch.Tensor, vcache: torch.Tensor, scores: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+             dst_tables: torch.Tensor, *, keep: int, recent: int, max_ctx: int, prefix_len: int = 0,
+             kept: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None):
+    """Per sequence and KV head: of the tokens behind prefix_len the last `recent` and the best-scored others, `keep` in all,
+    copied in order with their scores to the pages of dst_tables (other pages of the same cache).  Returns (kept positions
+    [B][Hkv][keep], -1 behind the last; new context lengths [B]).  m355_kv_evict."""
+    _one_device(kcache=kcache, vcache=vcache, scores=scores, block_tables=block_tables, ctx_lens=ctx_lens, dst_tables=dst_tables, kept=kept,
+                new_lens=new_lens)
+    B, max_blocks = block_tables.shape
+    nblocks, block_size, Hkv, D = kcache.shape
+    if ctx_lens.numel() != B or dst_tables.shape[0] != B:
+        raise ValueError(f"block_tables has {B} rows, ctx_lens {ctx_lens.numel()} entries, dst_tables {dst_tables.shape[0]} rows")
+    stride, size = _paged_cache(kcache, vcache, kcache.dtype), kcache.element_size()
+    if kept is None:
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=kcache.device)
+    elif tuple(kept.shape) != (B, Hkv, keep):
+        raise ValueError(f"kept is {tuple(kept.shape)}, expected {(B, Hkv, keep)}")
+    if new_lens is None:
+        new_lens = torch.empty((B,), dtype=torch.int32, device=kcache.device)
+    elif new_lens.numel() != B:
+        raise ValueError(f"new_lens has {new_lens.numel()} entries, expected {B}")
+    _check(load().m355_kv_evict(
+        kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _dev(block_tables, torch.int32, "block_tables"),
+        _dev(ctx_lens, torch.int32, "ctx_lens"), _dev(dst_tables, torch.int32, "dst_tables"), B, Hkv, D * size, nblocks, block_size,
+        max_blocks, dst_tables.shape[1], stride * size, int(max_ctx), int(prefix_len), int(keep), int(recent), _dev(kept, torch.int32, "kept"),
+        _dev(new_lens, torch.int32, "new_lens"), _stream()), "m355_kv_evict")
+    return kept, new_lens

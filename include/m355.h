@@ -32,6 +32,9 @@ typedef void* m355_stream_t; /* a hipStream_t (NULL = the default stream) */
                                   h = (up + 1) * gate * sigmoid(alpha * gate) (GptOssExperts._apply_gate,
                                   transformers models/gpt_oss/modeling_gpt_oss.py:79-85); the reference replaces it
                                   with plain silu (patches/unsloth_to_vllm_converter.py:312-315) */
+/* dtype of the entry points that take more than fp16 */
+#define M355_DTYPE_F16 0
+#define M355_DTYPE_BF16 1
 /* flags of m355_moe_nf4_forward */
 #define M355_FLAG_FP16_COMBINE 1 /* routing weights rounded to fp16 and out accumulated over k in fp16, in
                                     k order, as the reference's fp16 tensors do
@@ -359,6 +362,65 @@ M355_API int m355_norm_qkv_rope_kv_write(const void* x_f16, const void* delta_f1
                                          int block_size, int max_pos, void* resid_out_f16, void* h_scratch_f16,
                                          void* qkv_scratch_f16, void* q_out_f16, void* kcache_f16, void* vcache_f16,
                                          m355_stream_t stream);
+
+/*
+ * Long contexts: attention of a batch that shares a prefix, the decode attention that accumulates what every cached token
+ * weighs, and eviction by that weight.  No counterpart in the reference (its attention is vLLM's FlashAttention-2 backend,
+ * patches/patch_2_force_fa2.py; --max-model-len 256, patches/gpt_oss_server.py); they extend m355_paged_attn_decode_ex and
+ * m355_attn_prefill, whose arithmetic (scale, sinks, window) they share.  dtype: M355_DTYPE_F16 or _BF16 for q, the caches,
+ * sinks and out.  D 64 or 128, any Hq that is a multiple of Hkv, any page size.  Caches [num_blocks][block_size][Hkv][D],
+ * pages block_stride elements apart (a multiple of 8); table entries outside [0, num_blocks) are clamped (no access leaves
+ * the cache; such a result has no meaning).  ctx_lens count the new tokens and are clamped to max_ctx (host).
+ *
+ * m355_shared_prefix_attn: new tokens q [T][Hq][D] (token stride q_stride) against the cache.  seq_starts [B + 1] (device):
+ *   first tokens of the sequences, max_q (host) the longest one's number of tokens; NULL: one token per sequence (T == B).
+ *   A sequence's n new tokens are the last n of its ctx_lens positions and see the keys up to their own (window > 0: the
+ *   last `window` of them).  The first prefix_len positions (host; 0: none) are the same tokens for every sequence: they are
+ *   read through row 0 of block_tables, once for all, the others through the sequence's own row.  prefix_len need not end a
+ *   page.  Queries may lie anywhere (a prefix_len beyond a sequence's end only hides what it does not see).  Rows that see
+ *   nothing become 0; rows of q behind seq_starts[B], and a sequence's tokens behind max_q, leave `out` as it was.
+ *   Infinities and NaN in K or V reach the queries that see them and no others.
+ *   With one sequence per row and prefix_len = 0 it is m355_paged_attn_decode_ex.
+ */
+M355_API int m355_shared_prefix_attn(const void* q, const void* kcache, const void* vcache, const int32_t* block_tables,
+                                     const int32_t* ctx_lens, const int32_t* seq_starts, int T, int B, int max_q, int Hq,
+                                     int Hkv, int D, int dtype, int num_blocks, int block_size, int max_blocks,
+                                     int64_t block_stride, int max_ctx, int prefix_len, int64_t q_stride, int64_t o_stride,
+                                     float scale, const void* sinks, int window, void* workspace, size_t ws_bytes, void* out,
+                                     m355_stream_t stream);
+M355_API size_t m355_shared_prefix_attn_workspace_bytes(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx,
+                                                        int prefix_len);
+/*
+ * m355_paged_attn_decode_scored: m355_shared_prefix_attn for one token per sequence, which also adds every own token's
+ *   attention weight to `scores` [num_blocks][Hkv][block_size] fp32: for each position j >= prefix_len that the query sees,
+ *   scores[page of j][hk][offset of j] += sum over the KV head's query heads of exp(s_j) / (sum_i exp(s_i) + exp(sink)).
+ *   The caller zeroes a page's scores when it hands the page out (m355_kv_evict does so for the page it leaves half full).
+ *   Two sequences of one call must not share a page behind prefix_len (their additions would race).  The same bits on every
+ *   run.
+ */
+M355_API int m355_paged_attn_decode_scored(const void* q, const void* kcache, const void* vcache, float* scores,
+                                           const int32_t* block_tables, const int32_t* ctx_lens, int B, int Hq, int Hkv, int D,
+                                           int dtype, int num_blocks, int block_size, int max_blocks, int64_t block_stride,
+                                           int max_ctx, int prefix_len, int64_t q_stride, int64_t o_stride, float scale,
+                                           const void* sinks, int window, void* workspace, size_t ws_bytes, void* out,
+                                           m355_stream_t stream);
+M355_API size_t m355_paged_attn_decode_scored_workspace_bytes(int B, int Hq, int Hkv, int D, int max_ctx, int prefix_len);
+/*
+ * m355_kv_evict: per sequence and KV head, of the own tokens (positions prefix_len .. ctx_lens[b] - 1) the last `recent`
+ *   are kept and of the others those with the largest scores (equal ones: the lower position; NaN counts as the smallest),
+ *   `keep` in all; fewer own tokens than that are all kept.  Their K and V rows and their scores are copied, in order, to
+ *   positions prefix_len .. of dst_tables [B][max_dst_blocks]: pages of the same cache that no sequence of the call reads
+ *   behind prefix_len (pages of the prefix stay shared and are not touched; prefix_len is a multiple of block_size).  The
+ *   source pages stay as they are, for the caller to release.  kept [B][Hkv][keep] receives the kept positions in order
+ *   (-1 behind them), new_lens [B] the new context length (prefix_len + kept tokens; a sequence that ends inside the prefix
+ *   keeps its length).  Scores of the rows behind the last kept token in its page become 0.  row_bytes: bytes of one token's
+ *   row of one KV head (D * element size, a multiple of 16); block_stride_bytes: bytes from page to page of kcache / vcache.
+ *   A destination entry outside [0, num_blocks) drops the rows that it would receive.
+ */
+M355_API int m355_kv_evict(void* kcache, void* vcache, float* scores, const int32_t* block_tables, const int32_t* ctx_lens,
+                           const int32_t* dst_tables, int B, int Hkv, int row_bytes, int num_blocks, int block_size,
+                           int max_blocks, int max_dst_blocks, int64_t block_stride_bytes, int max_ctx, int prefix_len,
+                           int keep, int recent, int32_t* kept, int32_t* new_lens, m355_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,380 @@
+"""Attention over a shared prefix, decode attention that accumulates token weights, eviction by that weight.
+
+The oracle is the formula in 64 bits, sequence by sequence on the CPU.  Tolerances: an output value is off by the rounding
+of its type (half a step, eps/2 relative), by the probabilities' rounding to that type before the second product (another
+eps/2 of sum p|v|, whatever their signs), and by the scores' own error: a 32-bit sum of D products of up to SMAX in size
+shifts an exponent by at most 2^-23 * D * SMAX, and the exponential and its argument's scaling add a few 2^-23 * SMAX.
+"""
+import numpy as np
+import pytest
+import torch
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+class Cache:
+    """A paged cache on the CPU with its tables; device() gives the GPU tensors."""
+
+    def __init__(self, seed, ctx, Hkv, D, block, dtype, prefix=0, spare=2, max_blocks=None, dst=0, poison=False, n=None, window=0):
+        g = torch.Generator().manual_seed(seed)
+        self.g, self.ctx, self.Hkv, self.D, self.block, self.dtype, self.prefix = g, list(ctx), Hkv, D, block, dtype, prefix
+        B = len(ctx)
+        pages = lambda n: (max(n, 0) + block - 1) // block      # noqa: E731
+        first = prefix // block
+        need = [max(0, pages(c) - first) for c in ctx]
+        dst_pages = max(0, pages(dst) - first) if dst else 0
+        total = pages(prefix) + sum(need) + B * dst_pages + spare
+        ids = torch.randperm(total, generator=g).tolist()
+        shared = [ids.pop() for _ in range(pages(prefix))]
+        width = max([pages(prefix)] + [pages(c) for c in ctx] + [1])
+        rows = []
+        for b in range(B):
+            row = shared[:first] + [ids.pop() for _ in range(need[b])]
+            if b == 0:
+                row = row[:first] + shared[first:] + row[len(shared):]
+            rows.append(row + [0] * (width - len(row)))
+        if max_blocks:
+            rows = [r + [0] * (max_blocks - len(r)) for r in rows]
+        self.tables = torch.tensor(rows, dtype=torch.int32)
+        self.dst = torch.tensor([shared[:first] + [ids.pop() for _ in range(dst_pages)] for _ in range(B)], dtype=torch.int32)
+        self.n = total
+        self.k = torch.randn((total, block, Hkv, D), generator=g).to(dtype)
+        self.v = torch.randn((total, block, Hkv, D), generator=g).to(dtype)
+        self.scores = torch.exp(torch.randn((total, Hkv, block), generator=g))
+        self.k_norm = float(self.k.float().norm(dim=-1).max())
+        if poison:                 # whatever no query sees holds NaN and infinities
+            seen = torch.zeros((total, block), dtype=torch.bool)
+            for b in range(B):
+                first_query = self.ctx[b] - (n[b] if n else 1)
+                page, off = self.slots(b, torch.arange(max(0, first_query - window + 1) if window else 0, max(self.ctx[b], 0)))
+                seen[page, off] = True
+            junk = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min]).to(dtype)
+            for t in (self.k, self.v):
+                fill = junk[torch.randint(0, 4, t.shape, generator=g)]
+                t[~seen] = fill[~seen]
+
+    def slots(self, b, positions=None):
+        pos = torch.arange(self.ctx[b]) if positions is None else positions
+        page = torch.where(pos < self.prefix, self.tables[0].long()[pos // self.block], self.tables[b].long()[pos // self.block])
+        return page, pos % self.block
+
+    def device(self, cuda):
+        return self.k.to(cuda), self.v.to(cuda), self.tables.to(cuda), torch.tensor(self.ctx, dtype=torch.int32, device=cuda)
+
+
+def oracle(c, q, n, scale, sinks=None, window=0):
+    """(out [T][Hq][D], sum p|v| of the same shape, own weights: list of [Hkv][ctx]) in 64 bits."""
+    T, Hq, D = q.shape
+    G = Hq // c.Hkv
+    out, mag, weights = torch.zeros((T, Hq, D), dtype=torch.float64), torch.zeros((T, Hq, D), dtype=torch.float64), []
+    t = 0
+    for b, nb in enumerate(n):
+        ctx = c.ctx[b]
+        page, off = c.slots(b)
+        k, v = c.k[page, off].double(), c.v[page, off].double()
+        w = torch.zeros((c.Hkv, max(ctx, 0)), dtype=torch.float64)
+        for j in range(nb):
+            pos = ctx - nb + j
+            lo = max(0, pos - window + 1) if window else 0
+            for h in range(Hq):
+                if pos < lo:
+                    continue
+                s = (k[lo:pos + 1, h // G] @ q[t + j, h].double()) * scale
+                m = s.max() if sinks is None else torch.maximum(s.max(), sinks[h].double())
+                e = torch.exp(s - m)
+                den = e.sum() + (0 if sinks is None else torch.exp(sinks[h].double() - m))
+                p = e / den
+                out[t + j, h] = p @ v[lo:pos + 1, h // G]
+                mag[t + j, h] = p @ v[lo:pos + 1, h // G].abs()
+                w[h // G, lo:pos + 1] += p
+        weights.append(w)
+        t += nb
+    return out, mag, weights
+
+
+def score_err(c, q, scale):
+    """Relative error of a probability, from the scores' rounding: see the module's docstring."""
+    smax = float(scale * q.float().norm(dim=-1).max()) * c.k_norm * 1.4427
+    return 2.0 ** -23 * (q.shape[-1] + 8) * max(smax, 1.0)
+
+
+def check(got, want, mag, dtype, rel):
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * half           # (fp16 results below the normal range round by a fixed step)
+    tol = half * want.abs() + (half + 2 * rel) * mag + 2 * tiny
+    err = (got.cpu().double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, worst {float((err / tol).max()):.2f} of the tolerance"
+
+
+LAYOUTS = [(64, 8, 64, F16), (8, 2, 128, BF16), (6, 2, 64, BF16), (5, 1, 128, F16), (3, 3, 64, F16), (40, 1, 64, F16), (66, 2, 64, BF16)]
+
+# own lengths, prefix, block, window, sinks
+DECODE = [
+    ([1], 0, 16, 0, False), ([1, 2, 33], 0, 16, 0, True), ([31, 32, 33, 64, 65], 7, 16, 0, False), ([1, 300], 257, 20, 0, True),
+    ([5, 1, 17], 1000, 16, 0, True), ([1, 9], 1, 1, 0, False), ([130, 1, 4], 333, 48, 128, True), ([1, 40], 64, 16, 1, False),
+    ([2, 700, 90], 31, 128, 600, False), ([0, 3, 0], 50, 16, 0, False), ([1, 2], 300, 16, 5, True),
+]
+
+
+def _inputs(c, T, Hq, seed, sinks):
+    g = torch.Generator().manual_seed(seed)
+    q = (1.5 * torch.randn((T, Hq, c.D), generator=g)).to(c.dtype)
+    return q, torch.randn((Hq,), generator=g).to(c.dtype) if sinks else None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS, ids=lambda x: f"{x[0]}-{x[1]}-{x[2]}-{str(x[3])[6:]}")
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_gpu_shared_prefix_decode(layout, case, m355, cuda):
+    """One token per sequence; everything no query sees is NaN or infinite."""
+    Hq, Hkv, D, dtype = layout
+    own, P, block, window, sinks = DECODE[case]
+    c = Cache(100 + case, [P + o for o in own], Hkv, D, block, dtype, prefix=P, poison=True, window=window)
+    q, sk = _inputs(c, len(own), Hq, case, sinks)
+    scale = D ** -0.5
+    want, mag, _ = oracle(c, q, [1] * len(own), scale, sk, window)
+    kc, vc, bt, cl = c.device(cuda)
+    for max_ctx in (max(c.ctx), c.tables.shape[1] * block):      # the bound may be loose
+        got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(max_ctx, 1), scale=scale,
+                                      sinks=None if sk is None else sk.to(cuda), window=window)
+        check(got, want, mag, dtype, score_err(c, q, scale))
+
+
+# own lengths, new tokens, prefix, block, window, sinks
+EXTEND = [
+    ([3], [3], 0, 16, 0, False), ([5, 1, 9, 4], [2, 1, 6, 0], 40, 16, 0, True), ([20, 33, 1], [20, 33, 1], 100, 32, 0, False),
+    ([70, 7], [65, 7], 31, 20, 9, True), ([2, 2, 50], [1, 2, 3], 200, 16, 0, False), ([40, 90], [7, 80], 129, 16, 64, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS[:6], ids=lambda x: f"{x[0]}-{x[1]}-{x[2]}-{str(x[3])[6:]}")
+@pytest.mark.parametrize("case", range(len(EXTEND)))
+def test_gpu_shared_prefix_several_tokens(layout, case, m355, cuda):
+    """Sequences with none to many new tokens; q is a strided slice, the cache's pages are strided, rows of q behind the
+    last sequence leave the output as it was."""
+    Hq, Hkv, D, dtype = layout
+    own, n, P, block, window, sinks = EXTEND[case]
+    c = Cache(300 + case, [P + o for o in own], Hkv, D, block, dtype, prefix=P, poison=True, n=n, window=window)
+    T, extra = sum(n), 3
+    q, sk = _inputs(c, T + extra, Hq, case, sinks)
+    scale = 0.7 * D ** -0.5
+    want, mag, _ = oracle(c, q[:T], n, scale, sk, window)
+    kv = torch.stack([c.k, c.v], dim=1).to(cuda)                          # K and V of a page side by side
+    fused = torch.full((T + extra, (Hq + 3) * D), 7.0, dtype=dtype, device=cuda)
+    fused[:, :Hq * D] = q.view(T + extra, -1).to(cuda)
+    _, _, bt, cl = c.device(cuda)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(n)]), dtype=torch.int32, device=cuda)
+    out = torch.full((T + extra, Hq + 1, D), -3.0, dtype=dtype, device=cuda)
+    got = m355.shared_prefix_attn(fused.view(T + extra, Hq + 3, D)[:, :Hq], kv[:, 0], kv[:, 1], bt, cl, prefix_len=P, max_ctx=max(c.ctx),
+                                  scale=scale, seq_starts=starts, max_q=max(n), sinks=None if sk is None else sk.to(cuda), window=window,
+                                  out=out[:, :Hq])
+    check(got[:T], want, mag, dtype, score_err(c, q, scale))
+    assert (out[T:] == -3.0).all() and (out[:, Hq:] == -3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_gpu_nonfinite_values_reach_only_who_sees_them(dtype, value, m355, cuda):
+    """The last of four drafted tokens of one sequence has a value row that is not finite: only its own query, the others'
+    formula is untouched; the same in the last prefix token under a window that only the shorter sequence still sees."""
+    c = Cache(5, [90, 100], 2, 64, 16, dtype, prefix=64)
+    q, _ = _inputs(c, 8, 8, 3, False)
+    n = [4, 4]
+    want, mag, _ = oracle(c, q, n, 0.125)
+    page, off = c.slots(0)
+    c.v[page[89], off[89], 1, 5] = value
+    kc, vc, bt, cl = c.device(cuda)
+    st = torch.tensor([0, 4, 8], dtype=torch.int32, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=64, max_ctx=100, scale=0.125, seq_starts=st, max_q=4).cpu()
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    hit[3, 4:, 5] = True
+    exp = torch.full((), value).to(dtype)
+    assert torch.equal(got[hit].isnan(), exp.expand(4).isnan()) and (exp.isnan() or (got[hit] == exp).all())
+    check(torch.where(hit, torch.zeros_like(got), got), torch.where(hit, 0.0, want), mag, dtype, score_err(c, q, 0.125))
+    # window 30: queries 86..89 of sequence 0 see prefix tokens 57.. / 60.., sequence 1's (96..99) none
+    c = Cache(6, [90, 100], 2, 64, 16, dtype, prefix=64)
+    want, mag, _ = oracle(c, q, n, 0.125, window=30)
+    page, off = c.slots(0)
+    c.v[page[58], off[58], 0, 63] = value
+    kc, vc, bt, cl = c.device(cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=64, max_ctx=100, scale=0.125, seq_starts=st, max_q=4, window=30).cpu()
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    hit[:2, :4, 63] = True
+    assert (~got[hit].isfinite()).all()
+    check(torch.where(hit, torch.zeros_like(got), got), torch.where(hit, 0.0, want), mag, dtype, score_err(c, q, 0.125))
+
+
+SCORED = [([1], 0, 16, 0, False), ([1, 2, 33], 0, 16, 0, True), ([31, 300, 65], 7, 16, 0, False), ([700, 5], 64, 20, 0, True),
+          ([260, 900], 0, 64, 200, True), ([3, 40], 33, 16, 2, False), ([0, 4], 48, 16, 0, False), ([1500], 1, 128, 0, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS, ids=lambda x: f"{x[0]}-{x[1]}-{x[2]}-{str(x[3])[6:]}")
+@pytest.mark.parametrize("case", range(len(SCORED)))
+def test_gpu_scored_decode(layout, case, m355, cuda):
+    """Output and accumulated weights; two steps in a row add up; no other score moves; the same bits on another run."""
+    Hq, Hkv, D, dtype = layout
+    own, P, block, window, sinks = SCORED[case]
+    c = Cache(500 + case, [P + o for o in own], Hkv, D, block, dtype, prefix=P, poison=True, window=window)
+    q, sk = _inputs(c, len(own), Hq, case, sinks)
+    scale = D ** -0.5
+    want, mag, weights = oracle(c, q, [1] * len(own), scale, sk, window)
+    kc, vc, bt, cl = c.device(cuda)
+    rel = score_err(c, q, scale)
+    steps = [c.scores.to(cuda), c.scores.to(cuda)]
+    for sc in steps:
+        for step in (1, 2):
+            got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, max_ctx=max(c.ctx), scale=scale, prefix_len=P,
+                                                sinks=None if sk is None else sk.to(cuda), window=window)
+            check(got, want, mag, dtype, rel)
+            exp, tol = c.scores.double().clone(), torch.zeros(c.scores.shape, dtype=torch.float64)
+            for b in range(len(own)):
+                page, off = c.slots(b)
+                w = weights[b].t()[P:]                                              # [own][Hkv]
+                exp[page[P:], :, off[P:]] += step * w
+                # every step: G weights of relative error rel and their sums, then a rounded addition
+                tol[page[P:], :, off[P:]] = step * (2 * rel + 2.0 ** -23 * (Hq // Hkv)) * w
+            tol += 2 * 2.0 ** -23 * exp * (tol > 0)
+            err = (sc.cpu().double() - exp).abs()
+            assert (err <= tol).all(), f"scores off by up to {float((err - tol).max()):.3g} over the tolerance"
+    assert torch.equal(*steps)
+
+
+EVICT = [([1], 0, 16, 4, 1), ([5, 6, 7], 0, 16, 6, 2), ([100, 300, 129], 32, 16, 64, 10), ([1000, 17], 0, 20, 33, 33),
+         ([700, 300], 64, 64, 256, 0), ([4, 2], 16, 16, 1, 0), ([3000, 64], 0, 128, 1025, 100), ([0, 9], 48, 16, 8, 3)]
+
+
+def evict_oracle(c, keep, recent):
+    kept, lens = torch.full((len(c.ctx), c.Hkv, keep), -1, dtype=torch.int32), []
+    for b, ctx in enumerate(c.ctx):
+        n = ctx - c.prefix
+        m = min(max(n, 0), keep)
+        lens.append(c.prefix + m if n > 0 else ctx)
+        page, off = c.slots(b)
+        for h in range(c.Hkv):
+            s = c.scores[page, h, off].tolist()[c.prefix:]
+            last = list(range(max(0, n - recent), n)) if n > keep else []
+            rest = [i for i in range(max(n, 0)) if i not in set(last)]
+            rest.sort(key=lambda i: (-float("inf") if s[i] != s[i] else s[i], s[i] == s[i], -i), reverse=True)
+            pick = sorted(rest[:m - len(last)] + last)
+            kept[b, h, :m] = torch.tensor(pick, dtype=torch.int32) + c.prefix
+    return kept, lens
+
+
+def _scores_at(c, kind):
+    s = c.scores
+    if kind == "ties":
+        s = torch.randint(0, 3, s.shape, generator=c.g).float()
+    elif kind == "special":
+        pool = torch.tensor([float("nan"), float("inf"), -float("inf"), 0.0, -0.0, 1e-42, -1.0, 3.4e38, 1.0])
+        s = pool[torch.randint(0, len(pool), s.shape, generator=c.g)]
+    elif kind == "close":            # differ in the last bits only
+        s = (torch.full(s.shape, 0x3f800000, dtype=torch.int32) + torch.randint(0, 700, s.shape, generator=c.g, dtype=torch.int32)).view(torch.float32)
+    c.scores = s.contiguous()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["plain", "ties", "special", "close"])
+@pytest.mark.parametrize("case", range(len(EVICT)))
+def test_gpu_kv_evict(case, kind, m355, cuda):
+    """Kept positions, lengths, moved rows and scores, bit for bit; everything else in the cache stays as it was."""
+    own, P, block, keep, recent = EVICT[case]
+    Hkv, D, dtype = [(8, 64, F16), (2, 128, BF16), (3, 64, F16)][case % 3]
+    c = Cache(700 + case, [P + o for o in own], Hkv, D, block, dtype, prefix=P, dst=P + keep)
+    _scores_at(c, kind)
+    kept, lens = evict_oracle(c, keep, recent)
+    exp = [c.k.clone(), c.v.clone(), c.scores.clone()]
+    for b in range(len(own)):
+        m = lens[b] - P
+        if m <= 0:
+            continue
+        to = torch.arange(P, P + m)
+        tp, tf = c.dst[b].long()[to // block], to % block
+        exp[2][tp[-1], :, (P + m - 1) % block + 1:] = 0.0
+        for h in range(Hkv):
+            page, off = c.slots(b, kept[b, h, :m].long())
+            exp[0][tp, tf, h], exp[1][tp, tf, h], exp[2][tp, h, tf] = c.k[page, off, h], c.v[page, off, h], c.scores[page, h, off]
+    kc, vc, bt, cl = c.device(cuda)
+    sc, dst = c.scores.to(cuda), c.dst.to(cuda)
+    for _ in range(2):                          # the source pages stay: a second call does the same again
+        got_kept, got_lens = m355.kv_evict(kc, vc, sc, bt, cl, dst, keep=keep, recent=recent, prefix_len=P, max_ctx=max(c.ctx))
+        assert torch.equal(got_kept.cpu(), kept)
+        assert got_lens.tolist() == lens
+        for got, want in zip((kc, vc, sc), exp):
+            assert torch.equal(got.cpu().view(torch.int16 if got.element_size() == 2 else torch.int32),
+                               want.view(torch.int16 if want.element_size() == 2 else torch.int32))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# refusals: checked before anything is launched, so they run without a GPU (the addresses are never dereferenced)
+# ---------------------------------------------------------------------------------------------------------------------
+PTR = 0x10000
+
+
+def _attn_args(L, **kw):
+    a = dict(q=PTR, kc=PTR, vc=PTR, tables=PTR, ctx=PTR, starts=None, T=4, B=4, max_q=1, Hq=16, Hkv=2, D=64, dtype=0, num_blocks=9,
+             block_size=16, max_blocks=4, block_stride=16 * 2 * 64, max_ctx=64, prefix=20, q_stride=1024, o_stride=1024, scale=0.125,
+             sinks=None, window=0, ws=PTR, ws_bytes=1 << 40, out=PTR)
+    a.update(kw)
+    return list(a.values()) + [None]
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(q=None), -1), (dict(out=None), -1), (dict(tables=None), -1), (dict(dtype=2), -2), (dict(D=96), -2), (dict(D=0), -2), (dict(Hq=15), -2),
+    (dict(Hkv=0), -2), (dict(T=-1), -2), (dict(B=-1), -2), (dict(T=5), -2), (dict(max_q=0), -2), (dict(block_size=0), -2),
+    (dict(num_blocks=0), -2), (dict(max_blocks=3), -2), (dict(max_ctx=0), -2), (dict(prefix=-1), -2), (dict(window=-1), -2),
+    (dict(block_stride=16 * 2 * 64 - 8), -2), (dict(block_stride=16 * 2 * 64 + 4), -2), (dict(q_stride=1016), -2), (dict(q_stride=1028), -2),
+    (dict(o_stride=1000), -2), (dict(q=PTR + 8), -3), (dict(kc=PTR + 2), -3), (dict(ws=None), -6), (dict(ws_bytes=100), -6), (dict(ws=PTR + 4), -3),
+    (dict(max_ctx=(1 << 30) + 1, max_blocks=1 << 27), -2), (dict(T=1 << 27, B=1 << 27), -2),
+])
+def test_shared_prefix_attn_refuses(bad, code, m355):
+    L = m355.load()
+    assert L.m355_shared_prefix_attn(*_attn_args(L, **bad)) == code
+    assert b"m355_shared_prefix_attn" in L.m355_last_error()
+    args = _attn_args(L, **bad)
+    if args[5] is None and not {"T", "max_q"} & set(bad):        # the scored form has no seq_starts, T and max_q
+        scored = args[:3] + [PTR] + args[3:5] + [args[7]] + args[9:]
+        assert L.m355_paged_attn_decode_scored(*scored) == code
+        assert b"m355_paged_attn_decode_scored" in L.m355_last_error()
+
+
+def test_shared_prefix_attn_accepts_empty(m355):
+    L = m355.load()
+    assert L.m355_shared_prefix_attn(*_attn_args(L, T=0, starts=PTR)) == 0
+    assert L.m355_shared_prefix_attn(*_attn_args(L, T=0, B=0)) == 0
+    assert L.m355_paged_attn_decode_scored(PTR, PTR, PTR, None, PTR, PTR, 4, 16, 2, 64, 0, 9, 16, 4, 2048, 64, 0, 1024, 1024, 0.1, None, 0, PTR,
+                                           1 << 40, PTR, None) == -1
+    assert m355.shared_prefix_attn_workspace_bytes(0, 4, 1, 16, 2, 64, 100, 0) == 0
+    for prefix in (0, 1, 64, 100, 200):
+        assert m355.paged_attn_decode_scored_workspace_bytes(4, 16, 2, 64, 100, prefix) >= m355.shared_prefix_attn_workspace_bytes(4, 4, 1, 16, 2, 64, 100, prefix) > 0
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(kc=None), -1), (dict(kept=None), -1), (dict(B=-1), -2), (dict(Hkv=0), -2), (dict(row_bytes=24), -2), (dict(row_bytes=0), -2),
+    (dict(num_blocks=0), -2), (dict(max_blocks=3), -2), (dict(max_dst=1), -2), (dict(prefix=8), -2), (dict(prefix=-16), -2), (dict(keep=0), -2),
+    (dict(recent=-1), -2), (dict(recent=33), -2), (dict(stride=16 * 2 * 128 - 16), -2), (dict(stride=16 * 2 * 128 + 8), -2), (dict(kc=PTR + 8), -3),
+    (dict(max_ctx=(1 << 30) + 1, max_blocks=1 << 27), -2), (dict(B=1 << 29), -2), (dict(new_lens=PTR * 2), -2),
+])
+def test_kv_evict_refuses(bad, code, m355):
+    L = m355.load()
+    a = dict(kc=PTR, vc=PTR, scores=PTR, tables=PTR, ctx=PTR * 2, dst=PTR, B=4, Hkv=2, row_bytes=128, num_blocks=9, block_size=16, max_blocks=4,
+             max_dst=3, stride=16 * 2 * 128, max_ctx=64, prefix=16, keep=32, recent=4, kept=PTR, new_lens=PTR * 3)
+    assert L.m355_kv_evict(*dict(a, B=0).values(), None) == 0
+    a.update(bad)
+    assert L.m355_kv_evict(*a.values(), None) == code
+    assert b"m355_kv_evict" in L.m355_last_error()
+
+
+def test_wrappers_refuse_cpu_tensors(m355):
+    c = Cache(1, [20, 30], 2, 64, 16, F16, dst=16)
+    cl = torch.tensor(c.ctx, dtype=torch.int32)
+    q = torch.zeros((2, 8, 64), dtype=F16)
+    with pytest.raises(m355.Mi355LibraryError, match="GPU tensor"):
+        m355.shared_prefix_attn(q, c.k, c.v, c.tables, cl, prefix_len=0, max_ctx=32, scale=0.1)
+    with pytest.raises(m355.Mi355LibraryError, match="GPU tensor"):
+        m355.paged_attn_decode_scored(q, c.k, c.v, c.scores, c.tables, cl, max_ctx=32, scale=0.1)
+    with pytest.raises(m355.Mi355LibraryError, match="GPU tensor"):
+        m355.kv_evict(c.k, c.v, c.scores, c.tables, cl, c.dst, keep=16, recent=1, max_ctx=32)
