@@ -20,15 +20,16 @@ namespace m355 {
 
 constexpr int SA_THREADS = 256;
 constexpr int SA_WAVES = SA_THREADS / 64;
-constexpr int SA_KT = 32;   // keys per tile
+constexpr int SA_PAGES = 256;     // entries of a wave's slice of the page table
+constexpr float SA_LAZY = 6.0f;   // log2 units the running maximum may exceed the exponents' reference point
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef short sa_short4_t __attribute__((ext_vector_type(4)));
-typedef short sa_short8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef const u32x4_t __attribute__((address_space(3))) sa_lds_u4_t;
-typedef __attribute__((address_space(3))) sa_short4_t sa_lds_s4_t;
+typedef __attribute__((address_space(3))) void sa_lds_void_t;
+typedef const __attribute__((address_space(1))) void sa_glb_void_t;
 
 struct SharedAttnArgs {
     const void *q, *kc, *vc, *sinks;
@@ -38,7 +39,8 @@ struct SharedAttnArgs {
     int page_shift;
     int64_t block_stride, q_stride, o_stride;
     int prefix_len, max_ctx, max_q, window;
-    float scale2;                                // scale * log2(e): scores are in the units of exp2
+    float scale2;                                // |scale| * log2(e): scores are in the units of exp2
+    uint32_t q_sign;                             // flips q's signs when scale is negative
     int np, sp, ns, so;                          // ranges over the prefix / the own tokens, and their lengths
     float *part_o, *part_ml;                     // [np + ns][T * Hq][D], [np + ns][T * Hq][2]
     float *logits, *final_ml, *scores;           // scored form: [B][Hq][lstride], [B * Hq][2], the caller's [num_blocks][Hkv][block_size]
@@ -50,13 +52,6 @@ struct SharedAttnArgs {
 __device__ __forceinline__ int page_of(const SharedAttnArgs& a, int key) {
     return (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
 }
-// element offset of a key's row of KV head hk; a table entry outside the cache is clamped (no access leaves the cache)
-__device__ __forceinline__ int64_t key_row(const SharedAttnArgs& a, const int32_t* table, int key, int hk, int D) {
-    const int page = page_of(a, key);
-    const int blk = min(max(table[page], 0), a.num_blocks - 1);
-    return blk * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D;
-}
-
 // What a sequence's row range and positions are.  Everything is clamped to what the arguments allow.
 struct SeqSpan {
     int t0, n, ctx;   // first token, number of tokens, cached tokens
@@ -89,8 +84,16 @@ __device__ __forceinline__ int window_lo(const SharedAttnArgs& a, int pos) {
     return a.window > 0 ? max(pos - a.window + 1, 0) : 0;
 }
 
-__device__ __forceinline__ float swap_half(float v) {   // the value that lane ^ 32 holds
-    return __shfl_xor(v, 32, 64);
+// The larger of this lane's value and the one lane ^ 32 holds: one v_permlane32_swap, no LDS round trip.
+__device__ __forceinline__ float half_max(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
 }
 __device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
@@ -129,195 +132,339 @@ __device__ __forceinline__ bool split_nonfinite(u32x4_t v, u32x4_t& clean, u32x4
     return any;
 }
 
-// Where a 16-byte chunk of a K row and of a V row lies in its LDS tile: XOR-swizzled so that the 32 rows read together
-// (K: one chunk of each; V: the transposing read's 4 rows x 64 bytes) cover every bank.
-template <int D>
-__device__ __forceinline__ uint32_t k_at(int key, int chunk) {
-    return key * (D * 2) + ((chunk ^ (D == 64 ? (key >> 1) & 7 : key & 15)) << 4);
-}
-template <int D>
-__device__ __forceinline__ uint32_t v_at(int key, int chunk) {
-    return key * (D * 2) + ((chunk ^ ((D == 64 ? (key >> 1) & 1 : key & 3) << 2)) << 4);
+// Two probabilities rounded to the cache's type (to nearest even), packed; `sum` takes them on as they were rounded.
+template <typename E>
+__device__ __forceinline__ uint32_t pack_p(float p0, float p1, float& sum) {
+    if constexpr (__is_same(E, half_t)) {
+        const half2_t ph = {(half_t)p0, (half_t)p1};
+        sum = __builtin_amdgcn_fdot2(ph, half2_t{(half_t)1.0f, (half_t)1.0f}, sum, false);
+        return __builtin_bit_cast(uint32_t, ph);
+    } else {
+        const bf16x2_t ph = {(bf16_t)p0, (bf16_t)p1};
+        sum = __builtin_amdgcn_fdot2_f32_bf16(ph, bf16x2_t{(bf16_t)1.0f, (bf16_t)1.0f}, sum, false);
+        return __builtin_bit_cast(uint32_t, ph);
+    }
 }
 
-constexpr int lds_bytes(int D, int RW) { return (RW == 4 ? 1 : SA_WAVES) * 2 * SA_KT * D * 2; }
+// 16-byte chunk c of a tile's row `key` lies at chunk c ^ k_swz (K) or c ^ v_swz (V) of that row: the 32 rows read together
+// (K: one chunk of each; V: the transposing read's 4 rows x 64 bytes) then cover every bank.
+template <int D>
+__device__ __forceinline__ int k_swz(int key) { return D == 64 ? (key >> 1) & 7 : key & 15; }
+template <int D>
+__device__ __forceinline__ int v_swz(int key) { return (D == 64 ? (key >> 1) & 1 : key & 3) << 2; }
 
-// One workgroup: the rows [row0, row_end) of KV head hk (at most 32 * RW) over the keys [kbeg, kend) of `table`, of which
-// those from kfloor on may be read.
-// RW = 4: the waves hold 32 rows each and share the tiles.  RW = 1: one set of 32 rows; the waves take the tiles in turn,
-// each in LDS of its own, and are joined at the end.  pos / lo: position and lowest visible key of this lane's row.
-template <typename E, int D, int RW, bool SCORED>
-__device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* smem, int hk, int row0, int row_end, int pos, int lo,
-                                       const int32_t* table, int kbeg, int kend, int kfloor, int split, int own_b, int own_k0) {
-    constexpr int TILE = SA_KT * D * 2;   // bytes of one K (or V) tile
-    constexpr int STEPS = D / 16, DT = D / 32;
+// V^T fragments through the transposing read.  In assembly, waiting for them in the same block: for the builtin the compiler
+// waits until every load into LDS in flight has landed, the coming tiles' among them.  `at`: LDS addresses of the 32-column
+// pieces, OFF: the 16 keys' offset in the tile; fragment dt is o[2 dt], o[2 dt + 1] (keys + 0 .. 7, + 8 .. 15).
+template <int OFF, int ROW>
+__device__ __forceinline__ void read_v4(uint32_t a0, uint32_t a1, u32x2_t (&o)[4]) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3])
+        : "v"(a0), "v"(a1), "i"(OFF), "i"(OFF + 8 * ROW)
+        : "memory");
+}
+template <int OFF, int ROW>
+__device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, u32x2_t (&o)[8]) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]), "=&v"(o[4]), "=&v"(o[5]), "=&v"(o[6]), "=&v"(o[7])
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(OFF), "i"(OFF + 8 * ROW)
+        : "memory");
+}
+
+// Shape of a workgroup's walk.  RW = 4: every wave holds 32 * QT rows, tiles of 64 keys are shared.  RW = 1: one set of 32
+// rows, the waves take tiles of 32 keys in turn, each in LDS of its own.  NS tiles are in LDS or on their way.
+template <int D, int RW>
+struct Walk {
+    static constexpr int KT = RW == 4 ? 64 : 32;
+    static constexpr int STAGE = 2 * KT * D * 2;                             // bytes: K rows, V rows
+    static constexpr int NS = RW == 4 && D == 64 ? 3 : 2;
+    static constexpr int NI = KT * D * 2 / 1024 / (RW == 4 ? SA_WAVES : 1);  // load instructions of a wave for K (as many for V)
+    static constexpr int TILES = NS * STAGE * (RW == 4 ? 1 : SA_WAVES);
+    static constexpr int LDS = TILES + SA_WAVES * SA_PAGES * 4;              // and every wave's slice of the page table
+};
+
+// One workgroup: the rows [row0, row_end) of KV head hk (at most 32 * RW * QT) over the keys [kbeg, kend) of `table`, of
+// which those from kfloor on may be read.  pos / lo: position and lowest visible key of this lane's row(s).
+template <typename E, int D, int RW, int QT, bool SCORED>
+__device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* smem, int hk, int row0, int row_end, const int (&pos)[QT],
+                                       const int (&lo)[QT], const int32_t* table, int kbeg, int kend, int kfloor, int split, int own_b,
+                                       int own_k0) {
+    typedef Walk<D, RW> W;
+    constexpr int KT = W::KT, ROW = D * 2, STEPS = D / 16, DT = D / 32, NI = W::NI, AHEAD = W::NS - 1;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 31, hh = lane >> 5;
-    const int row = min(row0 + (RW == 4 ? 32 * wave : 0) + qi, row_end - 1);
-    const int token = row / a.G, head = hk * a.G + row % a.G;
-
-    u32x4_t qf[STEPS];   // B operand of step s: Q[row][16 s + 8 hh ..]
-    {
-        const E* qrow = reinterpret_cast<const E*>(a.q) + token * a.q_stride + head * D + 8 * hh;
+    int token[QT], head[QT];
+    bool mine[QT];
+    u32x4_t qf[QT][STEPS];   // B operand of step s: Q[row][16 s + 8 hh ..]
+    int pos_min = INT32_MAX, lo_max = 0;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) qf[s] = *reinterpret_cast<const u32x4_t*>(qrow + 16 * s);
+    for (int t = 0; t < QT; t++) {
+        const int r = row0 + (RW == 4 ? 32 * (wave * QT + t) : 0) + qi, row = min(r, row_end - 1);
+        mine[t] = r < row_end;
+        token[t] = row / a.G;
+        head[t] = hk * a.G + row % a.G;
+        const E* qrow = reinterpret_cast<const E*>(a.q) + token[t] * a.q_stride + head[t] * D + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            qf[t][s] = *reinterpret_cast<const u32x4_t*>(qrow + 16 * s);
+            qf[t][s] ^= a.q_sign;   // (a negative scale: scale2 is its magnitude)
+        }
+        pos_min = min(pos_min, wave_min_i(pos[t]));
+        lo_max = max(lo_max, -wave_min_i(-lo[t]));
     }
-    const int pos_min = wave_min_i(pos), lo_max = -wave_min_i(-lo);
-    unsigned char* kt = smem + (RW == 4 ? 0 : wave * 2 * TILE);
-    unsigned char* vt = kt + TILE;
-    const int dg = (lane >> 4) & 1, ga = (lane & 15) >> 2, gc = lane & 3;
 
-    float m_run = -INFINITY, l_run = 0.f;
-    f32x16_t o[DT];
+    unsigned char* tiles = smem + (RW == 4 ? 0 : wave * W::NS * W::STAGE);
+    const uint32_t tiles_at = (uint32_t)(uintptr_t)(sa_lds_void_t*)tiles;
+    // what this lane loads: chunk `lchunk` of row lrow of the 1024 bytes of each load instruction
+    constexpr int RPI = 1024 / ROW, LPR = 64 / RPI;
+    const int lrow = lane / LPR, lchunk = lane % LPR;
+    auto key_of = [&](int t) { return kbeg + KT * (RW == 4 ? t : wave + SA_WAVES * t); };   // first key of this wave's tile t
+    const int nt_all = (kend - kbeg + KT - 1) / KT, nt = RW == 4 ? nt_all : (nt_all - wave + SA_WAVES - 1) / SA_WAVES;
+    // The wave's slice of the page table, in LDS: look-ups then do not queue behind the rows' loads (which return in order)
+    int32_t* pages = reinterpret_cast<int32_t*>(smem + W::TILES) + wave * SA_PAGES;
+    int pages_from = 0, pages_to = 0;
+    // keys outside re-read the nearest one: they are masked below, and rows nobody may see are never read
+    auto readable = [&](int key) { return max(min(key, kend - 1), kfloor); };
+    auto stage = [&](int t) {
+        const int k_first = key_of(t);
+        if (page_of(a, readable(k_first + KT - 1)) >= pages_to) {   // (uniform; a tile spans at most KT < SA_PAGES pages)
+            pages_from = page_of(a, readable(k_first));
+            pages_to = pages_from + SA_PAGES;
+            const int last = page_of(a, readable(kend - 1));
+#pragma unroll
+            for (int i = 0; i < SA_PAGES; i += 64)   // (no access leaves the cache, whatever the table holds)
+                pages[i + lane] = min(max(table[min(pages_from + i + lane, last)], 0), a.num_blocks - 1);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        const int key = readable(k_first + (lane & (KT - 1))), page = page_of(a, key);   // lane l looks up key l
+        const int64_t off = pages[page - pages_from] * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D;
+        unsigned char* dst = tiles + (t % W::NS) * W::STAGE + (RW == 4 ? wave * NI * 1024 : 0);
+        int64_t src[NI];
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int row = ((RW == 4 ? wave * NI : 0) + i) * RPI + lrow;
+            const uint32_t lo32 = __shfl((int)(uint32_t)off, row, 64), hi32 = __shfl((int)(off >> 32), row, 64);
+            src[i] = (int64_t)(((uint64_t)hi32 << 32) | lo32);
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int row = ((RW == 4 ? wave * NI : 0) + i) * RPI + lrow;
+            __builtin_amdgcn_global_load_lds((sa_glb_void_t*)(reinterpret_cast<const E*>(a.kc) + src[i] + ((lchunk ^ k_swz<D>(row)) << 3)),
+                                             (sa_lds_void_t*)(dst + i * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int row = ((RW == 4 ? wave * NI : 0) + i) * RPI + lrow;
+            __builtin_amdgcn_global_load_lds((sa_glb_void_t*)(reinterpret_cast<const E*>(a.vc) + src[i] + ((lchunk ^ v_swz<D>(row)) << 3)),
+                                             (sa_lds_void_t*)(dst + KT * ROW + i * 1024), 16, 0, 0);
+        }
+    };
+
+    // A fragment of S^T step s: chunk 2 s + hh of key qi's row
+    uint32_t kat[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) kat[s] = qi * ROW + (((2 * s + hh) ^ k_swz<D>(qi)) << 4);
+    // V^T: lane 4 ga + gc of a 16-lane group supplies key 4 hh + ga, columns 4 gc .. of its 16; lane i receives column i
+    const int ga = (lane & 15) >> 2, gc = lane & 3, vkey = 4 * hh + ga;
+    uint32_t vat[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
+        vat[dt] = KT * ROW + vkey * ROW + (((4 * dt + 2 * ((lane >> 4) & 1) + (gc >> 1)) ^ v_swz<D>(vkey)) << 4) + 8 * (gc & 1);
 
-    for (int k0 = kbeg + (RW == 4 ? 0 : wave * SA_KT); k0 < kend; k0 += (RW == 4 ? SA_KT : SA_WAVES * SA_KT)) {
-        constexpr int CH = D / 8;                            // 16-byte chunks per row
-        constexpr int N = SA_KT * CH / (RW == 4 ? SA_THREADS : 64);
-        u32x4_t kr[N], vr[N];
-        const int first = RW == 4 ? tid : lane;
+    float m_run[QT], l_run[QT];   // reference point of the exponents; this lane's half of the denominator
+    f32x16_t o[QT][DT];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int c = first + i * (RW == 4 ? SA_THREADS : 64);
-            // keys outside re-read the nearest one: they are masked below, and rows nobody may see are never read
-            const int64_t at = key_row(a, table, max(min(k0 + c / CH, kend - 1), kfloor), hk, D) + (c % CH) * 8;
-            kr[i] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const E*>(a.kc) + at);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const E*>(a.vc) + at);
-        }
-        if (RW == 4) __syncthreads();   // the previous tile has been read
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int c = first + i * (RW == 4 ? SA_THREADS : 64);
-            *reinterpret_cast<u32x4_t*>(kt + k_at<D>(c / CH, c % CH)) = kr[i];
-            *reinterpret_cast<u32x4_t*>(vt + v_at<D>(c / CH, c % CH)) = vr[i];
-        }
-        if (RW == 4) {
-            __syncthreads();
-        } else {   // (LDS serves a wave's instructions in order; the fence keeps the compiler's order)
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-        f32x16_t x;
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) x = mma<E>(*(sa_lds_u4_t*)(kt + k_at<D>(qi, 2 * s + hh)), qf[s], x);
-        // register i: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] *= a.scale2;
-        const bool edge = k0 + SA_KT > kend || k0 + SA_KT - 1 > pos_min || k0 < lo_max;   // (uniform over the wave)
-        if (edge) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int key = k0 + (i & 3) + 8 * (i >> 2) + 4 * hh;
-                x[i] = (key < kend && key <= pos && key >= lo) ? x[i] : -INFINITY;
-            }
-        }
-        if constexpr (SCORED) {
-            if (own_k0 >= 0 && row0 + qi < row_end) {
-                float* dst = a.logits + ((int64_t)own_b * a.Hq + head) * a.lstride + (k0 - own_k0) + 4 * hh;
-#pragma unroll
-                for (int i4 = 0; i4 < 4; i4++)
-                    *reinterpret_cast<float4_t*>(dst + 8 * i4) = float4_t{x[4 * i4], x[4 * i4 + 1], x[4 * i4 + 2], x[4 * i4 + 3]};
-            }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < 16; i++) mx = fmaxf(mx, x[i]);
-        mx = fmaxf(mx, swap_half(mx));
-        const float m_new = fmaxf(m_run, mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;   // nothing visible so far: every term is 0
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-        float sum = 0.f;
-        E pf[2][8];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float p = __builtin_amdgcn_exp2f(x[i] - m_use);
-            sum += p;
-            pf[i >> 3][i & 7] = (E)p;
-        }
-        sum += swap_half(sum);
-        l_run = l_run * alpha + sum;
-        m_run = m_new;
+    for (int t = 0; t < QT; t++) {
+        m_run[t] = -INFINITY;
+        l_run[t] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
-        // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
+            for (int i = 0; i < 16; i++) o[t][dt][i] = 0.f;
+    }
+
 #pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-            u32x4_t pb;
-            __builtin_memcpy(&pb, pf[s2], 16);
+    for (int t = 0; t < AHEAD; t++)
+        if (t < nt) stage(t);
+    for (int t = 0; t < nt; t++) {
+        // This tile has landed: of the requests after it, those of AHEAD - 1 tiles may still be under way (behind the last
+        // request: none).  RW = 4: on every wave, and nobody reads the buffer that is filled next.
+        if (AHEAD > 1 && t + AHEAD <= nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((AHEAD - 1) * 2 * NI) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (RW == 4) asm volatile("s_barrier" ::: "memory");
+        if (t + AHEAD < nt) stage(t + AHEAD);
+        const uint32_t base = tiles_at + (t % W::NS) * W::STAGE;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                // lane 4 ga + gc of a 16-lane group supplies key 4 hh + ga, columns 4 gc ..; lane i receives column i
-                const int key = 16 * s2 + 4 * hh + ga, chunk = 4 * dt + 2 * dg + (gc >> 1);
-                const sa_short4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_lds_s4_t*)(vt + v_at<D>(key, chunk) + 8 * (gc & 1)));
-                const sa_short4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_lds_s4_t*)(vt + v_at<D>(key + 8, chunk) + 8 * (gc & 1)));
-                const sa_short8_t av8 = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                u32x4_t av = __builtin_bit_cast(u32x4_t, av8);
+        for (int sub = 0; sub < KT / 32; sub++) {
+            const int k0 = key_of(t) + 32 * sub;
+            if (sub && k0 >= kend) break;   // (uniform)
+            f32x16_t x[QT];
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) {
+                const u32x4_t kf = *reinterpret_cast<sa_lds_u4_t*>(base + kat[s] + sub * 32 * ROW);
+#pragma unroll
+                for (int q = 0; q < QT; q++) {
+                    const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    x[q] = mma<E>(kf, qf[q][s], s ? x[q] : z);
+                }
+            }
+            u32x2_t vf[DT == 2 ? 2 : 1][2 * DT];   // (the reads run while the matrix cores form the scores)
+            if constexpr (DT == 2) {
+                if (sub == 0) {
+                    read_v4<0, ROW>(base + vat[0], base + vat[1], vf[0]);
+                    read_v4<16 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
+                } else {
+                    read_v4<32 * ROW, ROW>(base + vat[0], base + vat[1], vf[0]);
+                    read_v4<48 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
+                }
+            } else {
+                if (sub == 0) read_v8<0, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+                else read_v8<32 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+            }
+            // register i of a lane: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
+            const bool edge = k0 + 32 > kend || k0 + 31 > pos_min || k0 < lo_max;   // (uniform over the wave)
+            uint32_t pb[QT][8], seen[QT];   // probabilities; bit i: register i's key is seen by this row
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                seen[q] = 0xffffu;
                 if (edge) {
-                    // 0 * inf is NaN: an infinite or NaN value of a token that some row does not see must not reach that row.
-                    // Such values are taken out of the product and counted instead, per row that sees them.
-                    u32x4_t clean, plus, minus;
-                    if (__any(split_nonfinite<E>(av, clean, plus, minus))) {
-                        constexpr uint32_t ONE = __is_same(E, half_t) ? 0x3c00u : 0x3f80u;
-                        u32x4_t seen;
+                    seen[q] = 0;
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            seen[j] = (x[8 * s2 + 2 * j] != -INFINITY ? ONE : 0u) | (x[8 * s2 + 2 * j + 1] != -INFINITY ? ONE << 16 : 0u);
-                        f32x16_t up, down;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) up[i] = down[i] = 0.f;
-                        up = mma<E>(plus, seen, up);
-                        down = mma<E>(minus, seen, down);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            if (up[i] > 0.f) o[dt][i] += INFINITY;
-                            if (down[i] > 0.f) o[dt][i] -= INFINITY;
-                        }
-                        av = clean;
+                    for (int i = 0; i < 16; i++) {
+                        const int key = k0 + (i & 3) + 8 * (i >> 2) + 4 * hh;
+                        const bool ok = key < kend && key <= pos[q] && key >= lo[q];
+                        x[q][i] = ok ? x[q][i] : -INFINITY;
+                        seen[q] |= ok ? 1u << i : 0u;
                     }
                 }
-                o[dt] = mma<E>(av, pb, o[dt]);
+                if constexpr (SCORED) {
+                    if (own_k0 >= 0 && mine[q]) {
+                        float* dst = a.logits + ((int64_t)own_b * a.Hq + head[q]) * a.lstride + (k0 - own_k0) + 4 * hh;
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; i4++)
+                            *reinterpret_cast<float4_t*>(dst + 8 * i4) = float4_t{x[q][4 * i4], x[q][4 * i4 + 1], x[q][4 * i4 + 2], x[q][4 * i4 + 3]} * a.scale2;
+                    }
+                }
+                float mx = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
+#pragma unroll
+                for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, x[q][i]), x[q][i + 1]);
+                mx = half_max(fmaxf(mx, x[q][15])) * a.scale2;
+                // The exponents' reference follows the running maximum lazily: it moves when a score exceeds it by more than
+                // SA_LAZY, so probabilities reach 2^SA_LAZY instead of 1 (every type holds them, and the denominator carries the
+                // same factor) and the outputs are rescaled a few times per row.  Until a row has seen a key it is -inf.
+                const bool move = m_run[q] == -INFINITY ? mx > -INFINITY : mx > m_run[q] + SA_LAZY;
+                if (__any(move)) {
+                    const float alpha = move ? __builtin_amdgcn_exp2f(m_run[q] - mx) : 1.0f;   // (0 for the first key)
+                    if (move) m_run[q] = mx;
+                    l_run[q] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[q][dt][i] *= alpha;
+                }
+                const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -ref));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -ref));
+                    float rounded = l_run[q];
+                    pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
+                    // (the accumulated weights are fp32: their denominator sums the unrounded terms)
+                    l_run[q] = SCORED ? l_run[q] + (p0 + p1) : rounded;
+                }
             }
-        }
-        if (RW != 4) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++) {
+                if constexpr (DT == 4) {
+                    if (s2 == 1) {
+                        if (sub == 0) read_v8<16 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+                        else read_v8<48 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const u32x2_t v0 = vf[DT == 2 ? s2 : 0][2 * dt], v1 = vf[DT == 2 ? s2 : 0][2 * dt + 1];
+                    const u32x4_t av = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+                    for (int q = 0; q < QT; q++) {
+                        const u32x4_t pv = {pb[q][4 * s2], pb[q][4 * s2 + 1], pb[q][4 * s2 + 2], pb[q][4 * s2 + 3]};
+                        if (edge) {
+                            // 0 * inf is NaN: an infinite or NaN value of a token that some row does not see must not reach
+                            // that row.  Such values are taken out of the product and counted instead, per row that sees them.
+                            u32x4_t clean, plus, minus;
+                            if (__any(split_nonfinite<E>(av, clean, plus, minus))) {
+                                constexpr uint32_t ONE = __is_same(E, half_t) ? 0x3c00u : 0x3f80u;
+                                u32x4_t ones;
+#pragma unroll
+                                for (int j = 0; j < 4; j++)
+                                    ones[j] = (seen[q] >> (8 * s2 + 2 * j) & 1 ? ONE : 0u) | (seen[q] >> (8 * s2 + 2 * j + 1) & 1 ? ONE << 16 : 0u);
+#pragma unroll
+                                for (int sign = 0; sign < 2; sign++) {
+                                    const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                                    const f32x16_t count = mma<E>(sign ? minus : plus, ones, z);
+#pragma unroll
+                                    for (int i = 0; i < 16; i++)
+                                        if (count[i] > 0.f) o[q][dt][i] += sign ? -INFINITY : INFINITY;
+                                }
+                                o[q][dt] = mma<E>(clean, pv, o[q][dt]);
+                                continue;
+                            }
+                        }
+                        o[q][dt] = mma<E>(av, pv, o[q][dt]);
+                    }
+                }
+            }
         }
     }
 
     const int64_t rows = (int64_t)a.T * a.Hq;
     if constexpr (RW == 4) {
-        if (row0 + 32 * wave + qi < row_end) {
-            const int64_t r = split * rows + (int64_t)token * a.Hq + head;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+        for (int q = 0; q < QT; q++) {
+            const float l = half_sum(l_run[q]);
+            if (mine[q]) {
+                const int64_t r = split * rows + (int64_t)token[q] * a.Hq + head[q];
 #pragma unroll
-                for (int i4 = 0; i4 < 4; i4++)
-                    *reinterpret_cast<float4_t*>(a.part_o + r * D + 32 * dt + 8 * i4 + 4 * hh) =
-                        float4_t{o[dt][4 * i4], o[dt][4 * i4 + 1], o[dt][4 * i4 + 2], o[dt][4 * i4 + 3]};
-            if (hh == 0) {
-                a.part_ml[r * 2] = m_run;
-                a.part_ml[r * 2 + 1] = l_run;
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; i4++)
+                        *reinterpret_cast<float4_t*>(a.part_o + r * D + 32 * dt + 8 * i4 + 4 * hh) =
+                            float4_t{o[q][dt][4 * i4], o[q][dt][4 * i4 + 1], o[q][dt][4 * i4 + 2], o[q][dt][4 * i4 + 3]};
+                if (hh == 0) {
+                    a.part_ml[r * 2] = m_run[q];
+                    a.part_ml[r * 2 + 1] = l;
+                }
             }
         }
     } else {
+        static_assert(QT == 1 && 32 * D * 4 <= W::NS * W::STAGE);
         __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
-        float* po = reinterpret_cast<float*>(smem) + wave * 32 * D;   // takes the place of the wave's tiles (same size)
+        auto po = [&](int w, int r) { return reinterpret_cast<float*>(smem + w * W::NS * W::STAGE) + r * D; };   // in place of the wave's tiles
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++)
-                *reinterpret_cast<float4_t*>(po + qi * D + 32 * dt + 8 * i4 + 4 * hh) =
-                    float4_t{o[dt][4 * i4], o[dt][4 * i4 + 1], o[dt][4 * i4 + 2], o[dt][4 * i4 + 3]};
+                *reinterpret_cast<float4_t*>(po(wave, qi) + 32 * dt + 8 * i4 + 4 * hh) =
+                    float4_t{o[0][dt][4 * i4], o[0][dt][4 * i4 + 1], o[0][dt][4 * i4 + 2], o[0][dt][4 * i4 + 3]};
+        const float lsum = half_sum(l_run[0]);
         if (hh == 0) {
-            wm[wave][qi] = m_run;
-            wl[wave][qi] = l_run;
+            wm[wave][qi] = m_run[0];
+            wl[wave][qi] = lsum;
         }
         __syncthreads();
         const int nrows = min(32, row_end - row0);
@@ -328,13 +475,11 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             for (int w = 1; w < SA_WAVES; w++) m = fmaxf(m, wm[w][r32]);
             float4_t tot = {0.f, 0.f, 0.f, 0.f};
             float l = 0.f;
-            if (m > -INFINITY) {
 #pragma unroll
-                for (int w = 0; w < SA_WAVES; w++) {
-                    const float f = __builtin_amdgcn_exp2f(wm[w][r32] - m);
-                    tot += f * *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(smem) + (w * 32 + r32) * D + d);
-                    l += f * wl[w][r32];
-                }
+            for (int w = 0; w < SA_WAVES; w++) {
+                const float f = wm[w][r32] == m ? 1.0f : __builtin_amdgcn_exp2f(wm[w][r32] - m);   // (nothing seen at all: 1 * 0)
+                tot += f * *reinterpret_cast<const float4_t*>(po(w, r32) + d);
+                l += f * wl[w][r32];
             }
             const int rr = row0 + r32;
             const int64_t r = split * rows + (int64_t)(rr / a.G) * a.Hq + hk * a.G + rr % a.G;
@@ -348,23 +493,30 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 }
 
 // The shared tokens: a workgroup per (row set, range, KV head).  All tokens' rows, in order.
-template <typename E, int D, int RW>
-__global__ __launch_bounds__(SA_THREADS) void shared_prefix_kernel(SharedAttnArgs a) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[lds_bytes(D, RW)];
+template <typename E, int D, int RW, int QT, bool SCORED>
+__global__ __launch_bounds__(SA_THREADS, 2) void shared_prefix_kernel(SharedAttnArgs a) {
+    constexpr int ROWS = 32 * RW * QT;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[Walk<D, RW>::LDS];
     __shared__ int ends[SA_WAVES][2];
-    const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, split = unit % a.np, row0 = unit / a.np * 32 * RW;
-    const int row_end = min(a.T * a.G, row0 + 32 * RW);
+    const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, split = unit % a.np, row0 = unit / a.np * ROWS;
+    const int row_end = min(a.T * a.G, row0 + ROWS);
     const int tid = threadIdx.x, wave = tid >> 6, qi = tid & 31;
-    const int row = min(row0 + (RW == 4 ? 32 * wave : 0) + qi, row_end - 1);
-    const int token = row / a.G, b = seq_of(a, token);
-    int pos = -1;
-    if (b >= 0) {
-        const SeqSpan s = seq_span(a, b);
-        pos = s.ctx - s.n + (token - s.t0);
+    int pos[QT], lo[QT], pos_max = -1, lo_min = INT32_MAX;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const int row = min(row0 + (RW == 4 ? 32 * (wave * QT + t) : 0) + qi, row_end - 1);
+        const int token = row / a.G, b = seq_of(a, token);
+        pos[t] = -1;
+        if (b >= 0) {
+            const SeqSpan s = seq_span(a, b);
+            pos[t] = s.ctx - s.n + (token - s.t0);
+        }
+        lo[t] = window_lo(a, pos[t]);
+        pos_max = max(pos_max, pos[t]);
+        if (pos[t] >= 0) lo_min = min(lo_min, lo[t]);
     }
-    const int lo = window_lo(a, pos);
     // the range's keys that any row of the workgroup sees
-    const int pos_max = -wave_min_i(-pos), lo_min = wave_min_i(pos >= 0 ? lo : INT32_MAX);
+    pos_max = -wave_min_i(-pos_max), lo_min = wave_min_i(lo_min);
     if ((tid & 63) == 0) {
         ends[wave][0] = lo_min;
         ends[wave][1] = pos_max;
@@ -378,13 +530,13 @@ __global__ __launch_bounds__(SA_THREADS) void shared_prefix_kernel(SharedAttnArg
     kbeg = max(kbeg, first);
     kend = min(kend, last + 1);
     if (kbeg >= kend) return;   // (the merge leaves out a range that a row does not see)
-    attend<E, D, RW, false>(a, smem, hk, row0, row_end, pos, lo, a.tables, kbeg, kend, kbeg, split, 0, -1);
+    attend<E, D, RW, QT, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables, kbeg, kend, kbeg, split, 0, -1);
 }
 
 // The sequences' own tokens: a workgroup per (sequence, row set of the longest sequence, range, KV head).
 template <typename E, int D, int RW, bool SCORED>
-__global__ __launch_bounds__(SA_THREADS) void own_tokens_kernel(SharedAttnArgs a, int row_sets) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[lds_bytes(D, RW)];
+__global__ __launch_bounds__(SA_THREADS, 2) void own_tokens_kernel(SharedAttnArgs a, int row_sets) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[Walk<D, RW>::LDS];
     const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, split = unit % a.ns;
     const int b = unit / a.ns / row_sets, set = unit / a.ns % row_sets;
     const SeqSpan s = seq_span(a, b);
@@ -393,55 +545,75 @@ __global__ __launch_bounds__(SA_THREADS) void own_tokens_kernel(SharedAttnArgs a
     const int tid = threadIdx.x, wave = tid >> 6, qi = tid & 31;
     const int row = min(row0 + (RW == 4 ? 32 * wave : 0) + qi, row_end - 1);
     const int pos0 = s.ctx - s.n - s.t0;                       // position of token t is pos0 + t
-    const int pos = pos0 + row / a.G, lo = window_lo(a, pos);
+    const int pos[1] = {pos0 + row / a.G}, lo[1] = {window_lo(a, pos[0])};
     const int k0 = a.prefix_len + split * a.so;
     const int kbeg = max(k0, window_lo(a, pos0 + row0 / a.G));
     const int kend = min(k0 + a.so, pos0 + (row_end - 1) / a.G + 1);
     if (kbeg >= kend) return;
     // (scored: the logits are addressed from the range's start in steps of a tile, so the walk starts on one)
-    const int aligned = SCORED ? k0 + (kbeg - k0) / SA_KT * SA_KT : kbeg;
-    attend<E, D, RW, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables + (int64_t)b * a.max_blocks, aligned, kend, kbeg,
-                             a.np + split, b, SCORED ? a.prefix_len : -1);
+    const int start = SCORED ? k0 + (kbeg - k0) / 32 * 32 : kbeg;
+    attend<E, D, RW, 1, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables + (int64_t)b * a.max_blocks, start, kend, kbeg,
+                                a.np + split, b, SCORED ? a.prefix_len : -1);
 }
 
-// Joins the ranges of one (token, query head).  One wave; a lane holds D / 64 columns.
+// Joins the ranges: a wave per (token, query head).  A lane looks after one range's (m, l), then the lanes stand D / 4 to a
+// range's row and 64 / (D / 4) ranges go by at a time.
 template <typename E, int D>
-__global__ __launch_bounds__(64) void shared_merge_kernel(SharedAttnArgs a) {
-    const int head = blockIdx.x % a.Hq, token = blockIdx.x / a.Hq, lane = threadIdx.x;
+__global__ __launch_bounds__(SA_THREADS) void shared_merge_kernel(SharedAttnArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hk = blockIdx.x % a.Hkv, row = blockIdx.x / a.Hkv * SA_WAVES + wave;   // (a KV head's rows stay on their chiplet)
+    if (row >= a.T * a.G) return;
+    const int token = row / a.G, head = hk * a.G + row % a.G;
     const int b = seq_of(a, token);
     if (b < 0) return;   // behind the last sequence: left as it was
     const SeqSpan s = seq_span(a, b);
     if (token - s.t0 >= a.max_q) return;
-    const int pos = s.ctx - s.n + (token - s.t0), lo = window_lo(a, pos);
+    const int pos = s.ctx - s.n + (token - s.t0), lo = window_lo(a, pos), n = a.np + a.ns;
     const int64_t rows = (int64_t)a.T * a.Hq, r = (int64_t)token * a.Hq + head;
-    auto live = [&](int i) {   // does this row see a key of range i?
+    constexpr int LPR = D / 4, GROUPS = 64 / LPR;
+    const int group = lane / LPR, col = (lane % LPR) * 4;
+    float m_run = -INFINITY, den = 0.f;
+    float4_t num = {0.f, 0.f, 0.f, 0.f};
+    if (a.sinks) {   // one more logit in the denominator
+        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
+        m_run = sk != sk ? 0.f : sk;
+        den = sk == -INFINITY ? 0.f : (sk != sk ? sk : 1.0f);
+    }
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
         const int beg = i < a.np ? i * a.sp : a.prefix_len + (i - a.np) * a.so;
         const int end = i < a.np ? min(beg + a.sp, a.prefix_len) : beg + a.so;
-        return max(beg, lo) < min(end, pos + 1);
-    };
-    float m = -INFINITY;
-    for (int i = 0; i < a.np + a.ns; i++)
-        if (live(i)) m = fmaxf(m, a.part_ml[(i * rows + r) * 2]);
-    float den = 0.f, num[D / 64] = {};
-    if (a.sinks) {
-        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
-        m = fmaxf(m, sk);
-        if (sk != -INFINITY) den = __builtin_amdgcn_exp2f(sk - m);
+        const bool live = i < n && max(beg, lo) < min(end, pos + 1);   // else this row sees none of its keys: nothing was written
+        float m = -INFINITY, l = 0.f;
+        if (live) {
+            m = a.part_ml[(i * rows + r) * 2];
+            l = a.part_ml[(i * rows + r) * 2 + 1];
+        }
+        const float m_new = fmaxf(m_run, wave_max(m));
+        const float back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        const float f = !live || l == 0.f ? 0.f : (m == m_new ? 1.0f : __builtin_amdgcn_exp2f(m - m_new));
+        den = den * back + wave_sum(f == 0.f && l == l ? 0.f : f * l);
+        num *= back;
+        m_run = m_new;
+        const int cnt = min(64, n - i0);
+#pragma unroll 4
+        for (int j = group; j < cnt; j += GROUPS) {
+            const float fj = __shfl(f, j, 64);
+            if (fj != 0.f) num += fj * *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
+        }
     }
-    for (int i = 0; i < a.np + a.ns; i++) {
-        if (!live(i)) continue;
-        const float l = a.part_ml[(i * rows + r) * 2 + 1];
-        if (l == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[(i * rows + r) * 2] - m);
-        den += f * l;
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) num[c] += f * a.part_o[(i * rows + r) * D + c * 64 + lane];
-    }
+    for (int st = LPR; st < 64; st *= 2)
+#pragma unroll
+        for (int c = 0; c < 4; c++) num[c] += __shfl_xor(num[c], st, 64);
     const float inv = den > 0.f ? 1.0f / den : (den == 0.f ? 0.f : den);   // (a NaN stays one)
+    if (group == 0) {
+        E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + col;
 #pragma unroll
-    for (int c = 0; c < D / 64; c++) reinterpret_cast<E*>(a.out)[token * a.o_stride + head * D + c * 64 + lane] = (E)(num[c] * inv);
+        for (int c = 0; c < 4; c++) out[c] = (E)(num[c] * inv);
+    }
     if (a.final_ml && lane == 0) {
-        a.final_ml[r * 2] = m == -INFINITY ? 0.f : m;
+        a.final_ml[r * 2] = m_run == -INFINITY ? 0.f : m_run;
         a.final_ml[r * 2 + 1] = inv;
     }
 }
@@ -465,7 +637,7 @@ __global__ __launch_bounds__(SA_THREADS) void score_add_kernel(SharedAttnArgs a,
 // ---------------------------------------------------------------------------------------------------------------------
 struct SharedAttnPlan {
     int np, sp, ns, so, lstride;
-    bool wide_prefix, wide_own;   // 128 rows per workgroup (RW = 4) instead of 32
+    int prefix_rows, own_rows;   // rows per workgroup: 32 (RW = 1), 128 or 256 (RW = 4)
     int64_t units;   // an upper bound of every launch's workgroups and row numbers
     size_t part_floats, logit_floats, bytes;
 };
@@ -473,8 +645,8 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     SharedAttnPlan p;
     max_q = max_q < T ? max_q : T;
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P;
-    p.wide_prefix = T * G > 32;
-    p.wide_own = max_q * G > 32 && !scored;
+    p.prefix_rows = T * G <= 32 ? 32 : D == 64 && T * G * Hkv >= 32768 && !scored ? 256 : 128;
+    p.own_rows = max_q * G > 32 && !scored ? 128 : 32;
     // ranges: enough workgroups for the chip, none shorter than 256 keys
     auto cut = [](int64_t keys, int64_t units, int& n, int& len) {
         n = 0, len = 256;
@@ -486,8 +658,8 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
         len = (int)l;
         n = (int)((keys + l - 1) / l);
     };
-    cut(P, (int64_t)Hkv * ((T * G + (p.wide_prefix ? 127 : 31)) / (p.wide_prefix ? 128 : 32)), p.np, p.sp);
-    cut(own, (int64_t)Hkv * B * ((max_q * G + (p.wide_own ? 127 : 31)) / (p.wide_own ? 128 : 32)), p.ns, p.so);
+    cut(P, (int64_t)Hkv * ((T * G + p.prefix_rows - 1) / p.prefix_rows), p.np, p.sp);
+    cut(own, (int64_t)Hkv * B * ((max_q * G + p.own_rows - 1) / p.own_rows), p.ns, p.so);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)((own + 127) / 128 * 128);
@@ -501,24 +673,22 @@ template <typename E, int D>
 static int launch_shared_attn(SharedAttnArgs& a, const SharedAttnPlan& p, bool scored, hipStream_t st) {
     const int rows = a.T * a.G;
     if (a.np) {
-        if (p.wide_prefix)
-            shared_prefix_kernel<E, D, 4><<<a.Hkv * a.np * ((rows + 127) / 128), SA_THREADS, 0, st>>>(a);
-        else
-            shared_prefix_kernel<E, D, 1><<<a.Hkv * a.np * ((rows + 31) / 32), SA_THREADS, 0, st>>>(a);
+        const int grid = a.Hkv * a.np * ((rows + p.prefix_rows - 1) / p.prefix_rows);
+        if (p.prefix_rows == 32 && scored) shared_prefix_kernel<E, D, 1, 1, true><<<grid, SA_THREADS, 0, st>>>(a);
+        else if (p.prefix_rows == 32) shared_prefix_kernel<E, D, 1, 1, false><<<grid, SA_THREADS, 0, st>>>(a);
+        else if (p.prefix_rows == 128 && scored) shared_prefix_kernel<E, D, 4, 1, true><<<grid, SA_THREADS, 0, st>>>(a);
+        else if (p.prefix_rows == 128) shared_prefix_kernel<E, D, 4, 1, false><<<grid, SA_THREADS, 0, st>>>(a);
+        else if constexpr (D == 64) shared_prefix_kernel<E, D, 4, 2, false><<<grid, SA_THREADS, 0, st>>>(a);
         M355_LAUNCH_CHECK("shared_prefix_kernel");
     }
     if (a.ns) {
-        const int per = p.wide_own ? 128 : 32, sets = (a.max_q * a.G + per - 1) / per;
-        const int grid = a.Hkv * a.ns * a.B * sets;
-        if (scored)
-            own_tokens_kernel<E, D, 1, true><<<grid, SA_THREADS, 0, st>>>(a, sets);
-        else if (p.wide_own)
-            own_tokens_kernel<E, D, 4, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
-        else
-            own_tokens_kernel<E, D, 1, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
+        const int sets = (a.max_q * a.G + p.own_rows - 1) / p.own_rows, grid = a.Hkv * a.ns * a.B * sets;
+        if (scored) own_tokens_kernel<E, D, 1, true><<<grid, SA_THREADS, 0, st>>>(a, sets);
+        else if (p.own_rows == 128) own_tokens_kernel<E, D, 4, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
+        else own_tokens_kernel<E, D, 1, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
         M355_LAUNCH_CHECK("own_tokens_kernel");
     }
-    shared_merge_kernel<E, D><<<a.Hq * a.T, 64, 0, st>>>(a);
+    shared_merge_kernel<E, D><<<a.Hkv * ((rows + SA_WAVES - 1) / SA_WAVES), SA_THREADS, 0, st>>>(a);
     M355_LAUNCH_CHECK("shared_merge_kernel");
     if (scored && a.ns) {
         const int pieces = (a.max_ctx - a.prefix_len + SA_THREADS - 1) / SA_THREADS;
@@ -563,7 +733,9 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     a.page_shift = 31 + sh;
     a.block_stride = block_stride, a.q_stride = q_stride, a.o_stride = o_stride;
     a.prefix_len = prefix_len < max_ctx ? prefix_len : max_ctx, a.max_ctx = max_ctx, a.max_q = max_q < T ? max_q : T, a.window = window;
-    a.scale2 = scale * 1.44269504088896341f;
+    // (never 0: a masked score, -inf, times 0 would be NaN; 1e-30 times any score is nothing)
+    a.scale2 = fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f);
+    a.q_sign = scale < 0.f ? 0x80008000u : 0u;
     a.np = p.np, a.sp = p.sp, a.ns = p.ns, a.so = p.so;
     a.part_o = reinterpret_cast<float*>(workspace);
     a.part_ml = a.part_o + (size_t)(p.np + p.ns) * T * Hq * D;
