@@ -16,6 +16,8 @@
 //                            operands; o and l stay fp32), are the B operand; V^T comes from LDS through the transposing read.
 #include "common.h"
 
+#include <type_traits>
+
 namespace m355 {
 
 constexpr int SA_THREADS = 256;
@@ -297,139 +299,157 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             for (int i = 0; i < 16; i++) o[t][dt][i] = 0.f;
     }
 
+    // 32 keys from k0 on, whose rows lie at LDS address `base` (K; V behind the tile's K rows).  EDGE: some row does not see
+    // some of them.
+    auto step = [&](auto edge_c, int k0, uint32_t base) {
+        constexpr bool EDGE = decltype(edge_c)::value;
+        const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        f32x16_t x[QT];
 #pragma unroll
-    for (int t = 0; t < AHEAD; t++)
-        if (t < nt) stage(t);
-    for (int t = 0; t < nt; t++) {
-        // This tile has landed: of the requests after it, those of AHEAD - 1 tiles may still be under way (behind the last
-        // request: none).  RW = 4: on every wave, and nobody reads the buffer that is filled next.
-        if (AHEAD > 1 && t + AHEAD <= nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((AHEAD - 1) * 2 * NI) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (RW == 4) asm volatile("s_barrier" ::: "memory");
-        if (t + AHEAD < nt) stage(t + AHEAD);
-        const uint32_t base = tiles_at + (t % W::NS) * W::STAGE;
+        for (int s = 0; s < STEPS; s++) {
+            const u32x4_t kf = *reinterpret_cast<sa_lds_u4_t*>(base + kat[s]);
 #pragma unroll
-        for (int sub = 0; sub < KT / 32; sub++) {
-            const int k0 = key_of(t) + 32 * sub;
-            if (sub && k0 >= kend) break;   // (uniform)
-            f32x16_t x[QT];
+            for (int q = 0; q < QT; q++) x[q] = mma<E>(kf, qf[q][s], s ? x[q] : zero);
+        }
+        u32x2_t vf[DT == 2 ? 2 : 1][2 * DT];   // (the reads run while the matrix cores form the scores)
+        if constexpr (DT == 2) {
+            read_v4<0, ROW>(base + vat[0], base + vat[1], vf[0]);
+            read_v4<16 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
+        } else {
+            read_v8<0, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+        }
+        // register i of a lane: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
+        uint32_t seen[QT];   // (EDGE) bit i: this row sees register i's key
+        float mx[QT];
+        bool move[QT], any = false;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const u32x4_t kf = *reinterpret_cast<sa_lds_u4_t*>(base + kat[s] + sub * 32 * ROW);
+        for (int q = 0; q < QT; q++) {
+            if constexpr (EDGE) {
+                seen[q] = 0;
 #pragma unroll
-                for (int q = 0; q < QT; q++) {
-                    const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    x[q] = mma<E>(kf, qf[q][s], s ? x[q] : z);
+                for (int i = 0; i < 16; i++) {
+                    const int key = k0 + (i & 3) + 8 * (i >> 2) + 4 * hh;
+                    const bool ok = key < kend && key <= pos[q] && key >= lo[q];
+                    x[q][i] = ok ? x[q][i] : -INFINITY;
+                    seen[q] |= ok ? 1u << i : 0u;
                 }
             }
-            u32x2_t vf[DT == 2 ? 2 : 1][2 * DT];   // (the reads run while the matrix cores form the scores)
-            if constexpr (DT == 2) {
-                if (sub == 0) {
-                    read_v4<0, ROW>(base + vat[0], base + vat[1], vf[0]);
-                    read_v4<16 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
-                } else {
-                    read_v4<32 * ROW, ROW>(base + vat[0], base + vat[1], vf[0]);
-                    read_v4<48 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
+            if constexpr (SCORED) {
+                if (own_k0 >= 0 && mine[q]) {
+                    float* dst = a.logits + ((int64_t)own_b * a.Hq + head[q]) * a.lstride + (k0 - own_k0) + 4 * hh;
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; i4++)
+                        *reinterpret_cast<float4_t*>(dst + 8 * i4) =
+                            float4_t{x[q][4 * i4], x[q][4 * i4 + 1], x[q][4 * i4 + 2], x[q][4 * i4 + 3]} * a.scale2;
                 }
-            } else {
-                if (sub == 0) read_v8<0, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
-                else read_v8<32 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
             }
-            // register i of a lane: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
-            const bool edge = k0 + 32 > kend || k0 + 31 > pos_min || k0 < lo_max;   // (uniform over the wave)
-            uint32_t pb[QT][8], seen[QT];   // probabilities; bit i: register i's key is seen by this row
+            mx[q] = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) mx[q] = fmaxf(fmaxf(mx[q], x[q][i]), x[q][i + 1]);
+            mx[q] = half_max(fmaxf(mx[q], x[q][15])) * a.scale2;
+            // The exponents' reference follows the running maximum lazily: it moves when a score exceeds it by more than
+            // SA_LAZY, so probabilities reach 2^SA_LAZY instead of 1 (every type holds them, and the denominator carries the
+            // same factor) and the outputs are rescaled a few times per row.  Until a row has seen a key it is -inf.
+            move[q] = m_run[q] == -INFINITY ? mx[q] > -INFINITY : mx[q] > m_run[q] + SA_LAZY;
+            any |= move[q];
+        }
+        if (__any(any)) {
 #pragma unroll
             for (int q = 0; q < QT; q++) {
-                seen[q] = 0xffffu;
-                if (edge) {
-                    seen[q] = 0;
+                float alpha = move[q] ? __builtin_amdgcn_exp2f(m_run[q] - mx[q]) : 1.0f;   // (0 for the first key)
+                asm volatile("" : "+v"(alpha));   // (keeps the multiplications below inside this rare branch)
+                if (move[q]) m_run[q] = mx[q];
+                l_run[q] *= alpha;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = k0 + (i & 3) + 8 * (i >> 2) + 4 * hh;
-                        const bool ok = key < kend && key <= pos[q] && key >= lo[q];
-                        x[q][i] = ok ? x[q][i] : -INFINITY;
-                        seen[q] |= ok ? 1u << i : 0u;
-                    }
-                }
-                if constexpr (SCORED) {
-                    if (own_k0 >= 0 && mine[q]) {
-                        float* dst = a.logits + ((int64_t)own_b * a.Hq + head[q]) * a.lstride + (k0 - own_k0) + 4 * hh;
+                for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                        for (int i4 = 0; i4 < 4; i4++)
-                            *reinterpret_cast<float4_t*>(dst + 8 * i4) = float4_t{x[q][4 * i4], x[q][4 * i4 + 1], x[q][4 * i4 + 2], x[q][4 * i4 + 3]} * a.scale2;
-                    }
-                }
-                float mx = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
-#pragma unroll
-                for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, x[q][i]), x[q][i + 1]);
-                mx = half_max(fmaxf(mx, x[q][15])) * a.scale2;
-                // The exponents' reference follows the running maximum lazily: it moves when a score exceeds it by more than
-                // SA_LAZY, so probabilities reach 2^SA_LAZY instead of 1 (every type holds them, and the denominator carries the
-                // same factor) and the outputs are rescaled a few times per row.  Until a row has seen a key it is -inf.
-                const bool move = m_run[q] == -INFINITY ? mx > -INFINITY : mx > m_run[q] + SA_LAZY;
-                if (__any(move)) {
-                    const float alpha = move ? __builtin_amdgcn_exp2f(m_run[q] - mx) : 1.0f;   // (0 for the first key)
-                    if (move) m_run[q] = mx;
-                    l_run[q] *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[q][dt][i] *= alpha;
-                }
-                const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -ref));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -ref));
-                    float rounded = l_run[q];
-                    pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
-                    // (the accumulated weights are fp32: their denominator sums the unrounded terms)
-                    l_run[q] = SCORED ? l_run[q] + (p0 + p1) : rounded;
-                }
+                    for (int i = 0; i < 16; i++) o[q][dt][i] *= alpha;
             }
-            // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
+        }
+        uint32_t pb[QT][8];
 #pragma unroll
-            for (int s2 = 0; s2 < 2; s2++) {
-                if constexpr (DT == 4) {
-                    if (s2 == 1) {
-                        if (sub == 0) read_v8<16 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
-                        else read_v8<48 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
-                    }
-                }
+        for (int q = 0; q < QT; q++) {
+            const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const u32x2_t v0 = vf[DT == 2 ? s2 : 0][2 * dt], v1 = vf[DT == 2 ? s2 : 0][2 * dt + 1];
-                    const u32x4_t av = {v0[0], v0[1], v1[0], v1[1]};
+            for (int i = 0; i < 16; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -ref));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -ref));
+                float rounded = l_run[q];
+                pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
+                // (the accumulated weights are fp32: their denominator sums the unrounded terms)
+                l_run[q] = SCORED ? l_run[q] + (p0 + p1) : rounded;
+            }
+        }
+        // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
 #pragma unroll
-                    for (int q = 0; q < QT; q++) {
-                        const u32x4_t pv = {pb[q][4 * s2], pb[q][4 * s2 + 1], pb[q][4 * s2 + 2], pb[q][4 * s2 + 3]};
-                        if (edge) {
-                            // 0 * inf is NaN: an infinite or NaN value of a token that some row does not see must not reach
-                            // that row.  Such values are taken out of the product and counted instead, per row that sees them.
-                            u32x4_t clean, plus, minus;
-                            if (__any(split_nonfinite<E>(av, clean, plus, minus))) {
-                                constexpr uint32_t ONE = __is_same(E, half_t) ? 0x3c00u : 0x3f80u;
-                                u32x4_t ones;
+        for (int s2 = 0; s2 < 2; s2++) {
+            if constexpr (DT == 4) {
+                if (s2 == 1) read_v8<16 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+            }
 #pragma unroll
-                                for (int j = 0; j < 4; j++)
-                                    ones[j] = (seen[q] >> (8 * s2 + 2 * j) & 1 ? ONE : 0u) | (seen[q] >> (8 * s2 + 2 * j + 1) & 1 ? ONE << 16 : 0u);
+            for (int dt = 0; dt < DT; dt++) {
+                const u32x2_t v0 = vf[DT == 2 ? s2 : 0][2 * dt], v1 = vf[DT == 2 ? s2 : 0][2 * dt + 1];
+                u32x4_t av = {v0[0], v0[1], v1[0], v1[1]};
+                if constexpr (EDGE) {
+                    // 0 * inf is NaN: an infinite or NaN value of a token that some row does not see must not reach that row.
+                    // Such values are taken out of the product and counted instead, per row that sees them.
+                    u32x4_t clean, plus, minus;
+                    if (__any(split_nonfinite<E>(av, clean, plus, minus))) {
+                        constexpr uint32_t ONE = __is_same(E, half_t) ? 0x3c00u : 0x3f80u;
+                        av = clean;
 #pragma unroll
-                                for (int sign = 0; sign < 2; sign++) {
-                                    const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                                    const f32x16_t count = mma<E>(sign ? minus : plus, ones, z);
+                        for (int q = 0; q < QT; q++) {
+                            u32x4_t ones;
 #pragma unroll
-                                    for (int i = 0; i < 16; i++)
-                                        if (count[i] > 0.f) o[q][dt][i] += sign ? -INFINITY : INFINITY;
-                                }
-                                o[q][dt] = mma<E>(clean, pv, o[q][dt]);
-                                continue;
+                            for (int j = 0; j < 4; j++)
+                                ones[j] = (seen[q] >> (8 * s2 + 2 * j) & 1 ? ONE : 0u) | (seen[q] >> (8 * s2 + 2 * j + 1) & 1 ? ONE << 16 : 0u);
+#pragma unroll
+                            for (int sign = 0; sign < 2; sign++) {
+                                const f32x16_t count = mma<E>(sign ? minus : plus, ones, zero);
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (count[i] > 0.f) o[q][dt][i] += sign ? -INFINITY : INFINITY;
                             }
                         }
-                        o[q][dt] = mma<E>(av, pv, o[q][dt]);
                     }
+                }
+#pragma unroll
+                for (int q = 0; q < QT; q++) {
+                    const u32x4_t pv = {pb[q][4 * s2], pb[q][4 * s2 + 1], pb[q][4 * s2 + 2], pb[q][4 * s2 + 3]};
+                    o[q][dt] = mma<E>(av, pv, o[q][dt]);
                 }
             }
         }
+    };
+
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++)
+        if (t < nt) stage(t);
+    // Tiles from t on as long as they are of the kind asked for; returns the next one.  (Two loops instead of a branch in one:
+    // across such a branch the compiler copies the outputs.)  Only tiles at a range's ends, a window's or a query's are EDGE.
+    auto is_edge = [&](int t) {   // (uniform over the wave)
+        const int k0 = key_of(t);
+        return k0 + KT > kend || k0 + KT - 1 > pos_min || k0 < lo_max;
+    };
+    auto tiles_of_kind = [&](auto edge_c, int t) {
+        constexpr bool EDGE = decltype(edge_c)::value;
+        for (; t < nt && is_edge(t) == EDGE; t++) {
+            // This tile has landed: of the requests after it, those of AHEAD - 1 tiles may still be under way (behind the last
+            // request: none).  RW = 4: on every wave, and nobody reads the buffer that is filled next.
+            if (AHEAD > 1 && t + AHEAD <= nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((AHEAD - 1) * 2 * NI) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if (RW == 4) asm volatile("s_barrier" ::: "memory");
+            if (t + AHEAD < nt) stage(t + AHEAD);
+            const int k0 = key_of(t);
+            const uint32_t base = tiles_at + (t % W::NS) * W::STAGE;
+#pragma unroll 1
+            for (int sub = 0; sub < KT && (!EDGE || k0 + sub < kend); sub += 32) step(edge_c, k0 + sub, base + sub * ROW);
+        }
+        return t;
+    };
+    for (int t = 0; t < nt;) {
+        t = tiles_of_kind(std::true_type{}, t);
+        t = tiles_of_kind(std::false_type{}, t);
     }
 
     const int64_t rows = (int64_t)a.T * a.Hq;
