@@ -64,6 +64,15 @@ int moe_static_device_init(int dev);
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// n / d for 0 <= n < 2^31 as (n * mul) >> shift in 64 bits, with mul = 2^shift / d rounded up and shift = 31 + ceil(log2 d):
+// the excess of mul over 2^shift / d is e / d with e < d <= 2^(shift - 31), so n * mul / 2^shift exceeds n / d by less than
+// n / (2^31 d) < 1 / d and cannot reach the next whole number.  mul fits 32 bits since d > 2^(shift - 32).
+inline void divide_by(int d, uint32_t& mul, int& shift) {
+    shift = 31;
+    while ((1ll << (shift - 31)) < d) shift++;
+    mul = (uint32_t)(((1ull << shift) + d - 1) / d);
+}
+
 // ---- device helpers ----
 // Reinterpret a dword as two fp16.  Always go through this by-value helper: __builtin_bit_cast applied
 // directly to an indexed vector element (v[j] with an unrolled loop index) was seen to read element 0

@@ -50,7 +50,7 @@ struct SharedAttnArgs {
     void* out;
 };
 
-// key / block_size for 0 <= key < 2^31: multiplication by a rounded-up reciprocal, exact in that range
+// key / block_size
 __device__ __forceinline__ int page_of(const SharedAttnArgs& a, int key) {
     return (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
 }
@@ -747,10 +747,7 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     a = SharedAttnArgs{};
     a.q = q, a.kc = kc, a.vc = vc, a.sinks = sinks, a.tables = tables, a.ctx_lens = ctx_lens, a.starts = starts;
     a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.num_blocks = num_blocks, a.block_size = block_size, a.max_blocks = max_blocks;
-    int sh = 0;
-    while ((1ll << sh) < block_size) sh++;
-    a.page_mul = (uint32_t)(((1ull << (31 + sh)) + block_size - 1) / block_size);
-    a.page_shift = 31 + sh;
+    divide_by(block_size, a.page_mul, a.page_shift);
     a.block_stride = block_stride, a.q_stride = q_stride, a.o_stride = o_stride;
     a.prefix_len = prefix_len < max_ctx ? prefix_len : max_ctx, a.max_ctx = max_ctx, a.max_q = max_q < T ? max_q : T, a.window = window;
     // (never 0: a masked score, -inf, times 0 would be NaN; 1e-30 times any score is nothing)
