@@ -23,6 +23,7 @@ namespace m355 {
 constexpr int SA_THREADS = 256;
 constexpr int SA_WAVES = SA_THREADS / 64;
 constexpr int SA_PAGES = 256;     // entries of a wave's slice of the page table
+constexpr float SA_NONE = -0x1p127f;   // "maximum" of a row that has seen no key: below every score, and finite
 constexpr float SA_LAZY = 6.0f;   // log2 units the running maximum may exceed the exponents' reference point
 
 typedef __bf16 bf16_t;
@@ -45,7 +46,7 @@ struct SharedAttnArgs {
     uint32_t q_sign;                             // flips q's signs when scale is negative
     int np, sp, ns, so;                          // ranges over the prefix / the own tokens, and their lengths
     float *part_o, *part_ml;                     // [np + ns][T * Hq][D], [np + ns][T * Hq][2]
-    float *logits, *final_ml, *scores;           // scored form: [B][Hq][lstride], [B * Hq][2], the caller's [num_blocks][Hkv][block_size]
+    float *logits, *scores;                      // scored form: [B][Hq][lstride], the caller's [num_blocks][Hkv][block_size]
     int lstride;
     void* out;
 };
@@ -97,10 +98,17 @@ __device__ __forceinline__ float half_sum(float v) {
     const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     return __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
 }
+// Wave-wide minimum with DPP only (lanes that a step leaves out combine with themselves).
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ int dpp_min(int v) { return min(v, __builtin_amdgcn_update_dpp(v, v, CTRL, ROW_MASK, 0xf, false)); }
 __device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    return __builtin_amdgcn_readfirstlane(v);
+    v = dpp_min<0xB1>(v);          // quad_perm [1,0,3,2]
+    v = dpp_min<0x4E>(v);          // quad_perm [2,3,0,1]
+    v = dpp_min<0x141>(v);         // row_half_mirror
+    v = dpp_min<0x140>(v);         // row_mirror: every lane holds its 16 lanes' minimum
+    v = dpp_min<0x142, 0xa>(v);    // row_bcast15 into rows 1 and 3
+    v = dpp_min<0x143, 0xc>(v);    // row_bcast31 into rows 2 and 3
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 template <typename E>
@@ -187,26 +195,43 @@ __device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t a2, u
         : "memory");
 }
 
-// Shape of a workgroup's walk.  RW = 4: every wave holds 32 * QT rows, tiles of 64 keys are shared.  RW = 1: one set of 32
-// rows, the waves take tiles of 32 keys in turn, each in LDS of its own.  NS tiles are in LDS or on their way.
+// Shape of a workgroup's walk.  RW = 4: every wave holds 32 * QT rows, tiles of 64 keys are shared, NS of them in LDS or on
+// their way.  RW = 1: one set of 32 rows, the waves take tiles of 32 keys in turn, each in LDS of its own; a tile is read
+// into registers whole, and the next one requested into its place before the softmax.
 template <int D, int RW>
 struct Walk {
     static constexpr int KT = RW == 4 ? 64 : 32;
     static constexpr int STAGE = 2 * KT * D * 2;                             // bytes: K rows, V rows
-    static constexpr int NS = RW == 4 && D == 64 ? 3 : 2;
+    static constexpr int NS = RW == 1 ? 1 : D == 64 ? 3 : 2;
     static constexpr int NI = KT * D * 2 / 1024 / (RW == 4 ? SA_WAVES : 1);  // load instructions of a wave for K (as many for V)
     static constexpr int TILES = NS * STAGE * (RW == 4 ? 1 : SA_WAVES);
     static constexpr int LDS = TILES + SA_WAVES * SA_PAGES * 4;              // and every wave's slice of the page table
 };
 
+// A wave's slice of the page table from page `from` on.  Entries behind the row's end repeat its last one, and an entry
+// outside the cache is clamped: no access leaves either, whatever the table holds.
+template <int D, int RW>
+__device__ __forceinline__ void fetch_pages(const SharedAttnArgs& a, unsigned char* smem, const int32_t* table, int from) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t* pages = reinterpret_cast<int32_t*>(smem + Walk<D, RW>::TILES) + wave * SA_PAGES;
+    int raw[SA_PAGES / 64];
+#pragma unroll
+    for (int i = 0; i < SA_PAGES / 64; i++) raw[i] = table[min(from + 64 * i + lane, a.max_blocks - 1)];
+#pragma unroll
+    for (int i = 0; i < SA_PAGES / 64; i++) pages[64 * i + lane] = min(max(raw[i], 0), a.num_blocks - 1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // One workgroup: the rows [row0, row_end) of KV head hk (at most 32 * RW * QT) over the keys [kbeg, kend) of `table`, of
-// which those from kfloor on may be read.  pos / lo: position and lowest visible key of this lane's row(s).
+// which those from kfloor on may be read.  pos / lo: position and lowest visible key of this lane's row(s).  The waves' table
+// slices hold the entries from pages_from on (fetch_pages).
 template <typename E, int D, int RW, int QT, bool SCORED>
 __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* smem, int hk, int row0, int row_end, const int (&pos)[QT],
-                                       const int (&lo)[QT], const int32_t* table, int kbeg, int kend, int kfloor, int split, int own_b,
-                                       int own_k0) {
+                                       const int (&lo)[QT], const int32_t* table, int pages_from, int kbeg, int kend, int kfloor,
+                                       int split, int own_b, int own_k0) {
     typedef Walk<D, RW> W;
-    constexpr int KT = W::KT, ROW = D * 2, STEPS = D / 16, DT = D / 32, NI = W::NI, AHEAD = W::NS - 1;
+    constexpr int KT = W::KT, ROW = D * 2, STEPS = D / 16, DT = D / 32, NI = W::NI, AHEAD = RW == 1 ? 1 : W::NS - 1;
+    constexpr int VH = RW == 4 && DT == 4 ? 1 : 2;   // V fragments of how many 16-key halves are read ahead of the softmax
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 31, hh = lane >> 5;
     int token[QT], head[QT];
@@ -237,20 +262,14 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
     auto key_of = [&](int t) { return kbeg + KT * (RW == 4 ? t : wave + SA_WAVES * t); };   // first key of this wave's tile t
     const int nt_all = (kend - kbeg + KT - 1) / KT, nt = RW == 4 ? nt_all : (nt_all - wave + SA_WAVES - 1) / SA_WAVES;
     // The wave's slice of the page table, in LDS: look-ups then do not queue behind the rows' loads (which return in order)
-    int32_t* pages = reinterpret_cast<int32_t*>(smem + W::TILES) + wave * SA_PAGES;
-    int pages_from = 0, pages_to = 0;
+    const int32_t* pages = reinterpret_cast<const int32_t*>(smem + W::TILES) + wave * SA_PAGES;
     // keys outside re-read the nearest one: they are masked below, and rows nobody may see are never read
     auto readable = [&](int key) { return max(min(key, kend - 1), kfloor); };
     auto stage = [&](int t) {
         const int k_first = key_of(t);
-        if (page_of(a, readable(k_first + KT - 1)) >= pages_to) {   // (uniform; a tile spans at most KT < SA_PAGES pages)
+        if (page_of(a, readable(k_first + KT - 1)) >= pages_from + SA_PAGES) {   // (uniform; a tile spans at most KT < SA_PAGES pages)
             pages_from = page_of(a, readable(k_first));
-            pages_to = pages_from + SA_PAGES;
-            const int last = page_of(a, readable(kend - 1));
-#pragma unroll
-            for (int i = 0; i < SA_PAGES; i += 64)   // (no access leaves the cache, whatever the table holds)
-                pages[i + lane] = min(max(table[min(pages_from + i + lane, last)], 0), a.num_blocks - 1);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            fetch_pages<D, RW>(a, smem, table, pages_from);
         }
         const int key = readable(k_first + (lane & (KT - 1))), page = page_of(a, key);   // lane l looks up key l
         const int64_t off = pages[page - pages_from] * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D;
@@ -291,7 +310,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
     f32x16_t o[QT][DT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        m_run[t] = -INFINITY;
+        m_run[t] = SA_NONE;
         l_run[t] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -300,8 +319,8 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
     }
 
     // 32 keys from k0 on, whose rows lie at LDS address `base` (K; V behind the tile's K rows).  EDGE: some row does not see
-    // some of them.
-    auto step = [&](auto edge_c, int k0, uint32_t base) {
+    // some of them.  RW = 1: tile t_next is requested as soon as this one has been read.
+    auto step = [&](auto edge_c, int k0, uint32_t base, int t_next) {
         constexpr bool EDGE = decltype(edge_c)::value;
         const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         f32x16_t x[QT];
@@ -311,12 +330,16 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 #pragma unroll
             for (int q = 0; q < QT; q++) x[q] = mma<E>(kf, qf[q][s], s ? x[q] : zero);
         }
-        u32x2_t vf[DT == 2 ? 2 : 1][2 * DT];   // (the reads run while the matrix cores form the scores)
+        u32x2_t vf[VH][2 * DT];   // (the reads run while the matrix cores form the scores)
         if constexpr (DT == 2) {
             read_v4<0, ROW>(base + vat[0], base + vat[1], vf[0]);
             read_v4<16 * ROW, ROW>(base + vat[0], base + vat[1], vf[1]);
         } else {
             read_v8<0, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
+            if constexpr (VH == 2) read_v8<16 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[1]);
+        }
+        if constexpr (RW == 1) {   // (those reads have returned, and K's before them)
+            if (t_next < nt) stage(t_next);
         }
         // register i of a lane: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
         uint32_t seen[QT];   // (EDGE) bit i: this row sees register i's key
@@ -349,8 +372,8 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             mx[q] = half_max(fmaxf(mx[q], x[q][15])) * a.scale2;
             // The exponents' reference follows the running maximum lazily: it moves when a score exceeds it by more than
             // SA_LAZY, so probabilities reach 2^SA_LAZY instead of 1 (every type holds them, and the denominator carries the
-            // same factor) and the outputs are rescaled a few times per row.  Until a row has seen a key it is -inf.
-            move[q] = m_run[q] == -INFINITY ? mx[q] > -INFINITY : mx[q] > m_run[q] + SA_LAZY;
+            // same factor) and the outputs are rescaled a few times per row.
+            move[q] = mx[q] > m_run[q] + SA_LAZY;
             any |= move[q];
         }
         if (__any(any)) {
@@ -369,11 +392,10 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         uint32_t pb[QT][8];
 #pragma unroll
         for (int q = 0; q < QT; q++) {
-            const float ref = m_run[q] == -INFINITY ? 0.f : m_run[q];
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -ref));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -ref));
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -m_run[q]));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -m_run[q]));
                 float rounded = l_run[q];
                 pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
                 // (the accumulated weights are fp32: their denominator sums the unrounded terms)
@@ -383,12 +405,12 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++) {
-            if constexpr (DT == 4) {
+            if constexpr (VH == 1) {
                 if (s2 == 1) read_v8<16 * ROW, ROW>(base + vat[0], base + vat[1], base + vat[2], base + vat[3], vf[0]);
             }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                const u32x2_t v0 = vf[DT == 2 ? s2 : 0][2 * dt], v1 = vf[DT == 2 ? s2 : 0][2 * dt + 1];
+                const u32x2_t v0 = vf[VH == 2 ? s2 : 0][2 * dt], v1 = vf[VH == 2 ? s2 : 0][2 * dt + 1];
                 u32x4_t av = {v0[0], v0[1], v1[0], v1[1]};
                 if constexpr (EDGE) {
                     // 0 * inf is NaN: an infinite or NaN value of a token that some row does not see must not reach that row.
@@ -439,11 +461,11 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             if (AHEAD > 1 && t + AHEAD <= nt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((AHEAD - 1) * 2 * NI) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             if (RW == 4) asm volatile("s_barrier" ::: "memory");
-            if (t + AHEAD < nt) stage(t + AHEAD);
+            if (RW == 4 && t + AHEAD < nt) stage(t + AHEAD);
             const int k0 = key_of(t);
             const uint32_t base = tiles_at + (t % W::NS) * W::STAGE;
 #pragma unroll 1
-            for (int sub = 0; sub < KT && (!EDGE || k0 + sub < kend); sub += 32) step(edge_c, k0 + sub, base + sub * ROW);
+            for (int sub = 0; sub < KT && (!EDGE || k0 + sub < kend); sub += 32) step(edge_c, k0 + sub, base + sub * ROW, t + 1);
         }
         return t;
     };
@@ -472,7 +494,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             }
         }
     } else {
-        static_assert(QT == 1 && 32 * D * 4 <= W::NS * W::STAGE);
+        static_assert(QT == 1 && 32 * D * 4 <= W::STAGE);
         __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
         auto po = [&](int w, int r) { return reinterpret_cast<float*>(smem + w * W::NS * W::STAGE) + r * D; };   // in place of the wave's tiles
 #pragma unroll
@@ -514,12 +536,12 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 
 // The shared tokens: a workgroup per (row set, range, KV head).  All tokens' rows, in order.
 template <typename E, int D, int RW, int QT, bool SCORED>
-__global__ __launch_bounds__(SA_THREADS, 2) void shared_prefix_kernel(SharedAttnArgs a) {
+__device__ __forceinline__ void prefix_part(const SharedAttnArgs& a, unsigned char* smem, int id) {
     constexpr int ROWS = 32 * RW * QT;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[Walk<D, RW>::LDS];
     __shared__ int ends[SA_WAVES][2];
-    const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, split = unit % a.np, row0 = unit / a.np * ROWS;
-    const int row_end = min(a.T * a.G, row0 + ROWS);
+    const int hk = id % a.Hkv, unit = id / a.Hkv, split = unit % a.np, row0 = unit / a.np * ROWS;
+    const int row_end = min(a.T * a.G, row0 + ROWS), pages_from = page_of(a, split * a.sp);
+    fetch_pages<D, RW>(a, smem, a.tables, pages_from);   // (needs nothing that is still to be looked up)
     const int tid = threadIdx.x, wave = tid >> 6, qi = tid & 31;
     int pos[QT], lo[QT], pos_max = -1, lo_min = INT32_MAX;
 #pragma unroll
@@ -537,28 +559,30 @@ __global__ __launch_bounds__(SA_THREADS, 2) void shared_prefix_kernel(SharedAttn
     }
     // the range's keys that any row of the workgroup sees
     pos_max = -wave_min_i(-pos_max), lo_min = wave_min_i(lo_min);
-    if ((tid & 63) == 0) {
-        ends[wave][0] = lo_min;
-        ends[wave][1] = pos_max;
+    if (RW == 4) {
+        if ((tid & 63) == 0) {
+            ends[wave][0] = lo_min;
+            ends[wave][1] = pos_max;
+        }
+        __syncthreads();
+        for (int w = 0; w < SA_WAVES; w++) {
+            lo_min = min(lo_min, ends[w][0]);
+            pos_max = max(pos_max, ends[w][1]);
+        }
     }
-    __syncthreads();
-    int kbeg = split * a.sp, kend = min(kbeg + a.sp, a.prefix_len), first = INT32_MAX, last = -1;
-    for (int w = 0; w < SA_WAVES; w++) {
-        first = min(first, ends[w][0]);
-        last = max(last, ends[w][1]);
-    }
-    kbeg = max(kbeg, first);
-    kend = min(kend, last + 1);
+    const int kbeg = max(split * a.sp, lo_min), kend = min(min(split * a.sp + a.sp, a.prefix_len), pos_max + 1);
     if (kbeg >= kend) return;   // (the merge leaves out a range that a row does not see)
-    attend<E, D, RW, QT, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables, kbeg, kend, kbeg, split, 0, -1);
+    attend<E, D, RW, QT, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables, pages_from, kbeg, kend, kbeg, split, 0, -1);
 }
 
 // The sequences' own tokens: a workgroup per (sequence, row set of the longest sequence, range, KV head).
 template <typename E, int D, int RW, bool SCORED>
-__global__ __launch_bounds__(SA_THREADS, 2) void own_tokens_kernel(SharedAttnArgs a, int row_sets) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[Walk<D, RW>::LDS];
-    const int hk = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv, split = unit % a.ns;
+__device__ __forceinline__ void own_part(const SharedAttnArgs& a, unsigned char* smem, int id, int row_sets) {
+    const int hk = id % a.Hkv, unit = id / a.Hkv, split = unit % a.ns;
     const int b = unit / a.ns / row_sets, set = unit / a.ns % row_sets;
+    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+    const int k0 = a.prefix_len + split * a.so, pages_from = page_of(a, k0);
+    fetch_pages<D, RW>(a, smem, table, pages_from);
     const SeqSpan s = seq_span(a, b);
     const int row0 = s.t0 * a.G + set * 32 * RW, row_end = min((s.t0 + s.n) * a.G, row0 + 32 * RW);
     if (row0 >= row_end) return;
@@ -566,22 +590,69 @@ __global__ __launch_bounds__(SA_THREADS, 2) void own_tokens_kernel(SharedAttnArg
     const int row = min(row0 + (RW == 4 ? 32 * wave : 0) + qi, row_end - 1);
     const int pos0 = s.ctx - s.n - s.t0;                       // position of token t is pos0 + t
     const int pos[1] = {pos0 + row / a.G}, lo[1] = {window_lo(a, pos[0])};
-    const int k0 = a.prefix_len + split * a.so;
     const int kbeg = max(k0, window_lo(a, pos0 + row0 / a.G));
     const int kend = min(k0 + a.so, pos0 + (row_end - 1) / a.G + 1);
     if (kbeg >= kend) return;
     // (scored: the logits are addressed from the range's start in steps of a tile, so the walk starts on one)
     const int start = SCORED ? k0 + (kbeg - k0) / 32 * 32 : kbeg;
-    attend<E, D, RW, 1, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables + (int64_t)b * a.max_blocks, start, kend, kbeg,
-                                a.np + split, b, SCORED ? a.prefix_len : -1);
+    attend<E, D, RW, 1, SCORED>(a, smem, hk, row0, row_end, pos, lo, table, pages_from, start, kend, kbeg, a.np + split, b,
+                                SCORED ? a.prefix_len : -1);
 }
 
-// Joins the ranges: a wave per (token, query head).  A lane looks after one range's (m, l), then the lanes stand D / 4 to a
-// range's row and 64 / (D / 4) ranges go by at a time.
+// Both in one launch: the prefix (bound by the matrix cores when there are many rows) and the own tokens (bound by memory)
+// run beside one another.
+template <typename E, int D, int RWP, int QT, int RWO, bool SCORED>
+__global__ __launch_bounds__(SA_THREADS, 2) void shared_attn_kernel(SharedAttnArgs a, int prefix_wgs, int row_sets) {
+    constexpr int LP = Walk<D, RWP>::LDS, LO = Walk<D, RWO>::LDS;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[LP > LO ? LP : LO];
+    if ((int)blockIdx.x < prefix_wgs) prefix_part<E, D, RWP, QT, SCORED>(a, smem, blockIdx.x);
+    else own_part<E, D, RWO, SCORED>(a, smem, blockIdx.x - prefix_wgs, row_sets);
+}
+
+// The ranges of one row, lane i looking after range i0 + i: does the row see a key of it (else nothing was written), and
+// its (m, l).
+struct RangeStat {
+    bool live;
+    float m, l;
+};
+__device__ __forceinline__ RangeStat range_stat(const SharedAttnArgs& a, int i, int64_t r, int pos, int lo) {
+    const int beg = i < a.np ? i * a.sp : a.prefix_len + (i - a.np) * a.so;
+    const int end = i < a.np ? min(beg + a.sp, a.prefix_len) : beg + a.so;
+    RangeStat s{i < a.np + a.ns && max(beg, lo) < min(end, pos + 1), SA_NONE, 0.f};
+    if (s.live) {
+        const float* ml = a.part_ml + (i * (int64_t)a.T * a.Hq + r) * 2;
+        s.m = ml[0];
+        s.l = ml[1];
+    }
+    return s;
+}
+template <typename E>
+__device__ __forceinline__ void start_with_sink(const SharedAttnArgs& a, int head, float& m, float& den) {
+    m = SA_NONE;
+    den = 0.f;
+    if (a.sinks) {   // one more logit in the denominator
+        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
+        m = sk > SA_NONE ? sk : SA_NONE;
+        den = sk == -INFINITY ? 0.f : sk == sk ? 1.0f : sk;   // (a NaN stays one)
+    }
+}
+// One 64 ranges' step of the running (m, den): returns this lane's factor (0: leave its range out).
+__device__ __forceinline__ float join_stats(const RangeStat& s, float& m_run, float& den, float& back) {
+    const float m_new = fmaxf(m_run, wave_max(s.m));
+    back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+    const float f = !s.live || s.l == 0.f ? 0.f : s.m == m_new ? 1.0f : __builtin_amdgcn_exp2f(s.m - m_new);
+    den = den * back + wave_sum(f == 0.f && s.l == s.l ? 0.f : f * s.l);
+    m_run = m_new;
+    return f;
+}
+__device__ __forceinline__ float inverse(float den) { return den > 0.f ? 1.0f / den : den == 0.f ? 0.f : den; }
+
+// Joins a row's ranges: a wave per (token, query head).  A lane looks after one range's (m, l), then the lanes stand D / 4 to
+// a range's row and 64 / (D / 4) ranges go by at a time.
 template <typename E, int D>
-__global__ __launch_bounds__(SA_THREADS) void shared_merge_kernel(SharedAttnArgs a) {
+__device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = blockIdx.x % a.Hkv, row = blockIdx.x / a.Hkv * SA_WAVES + wave;   // (a KV head's rows stay on their chiplet)
+    const int hk = id % a.Hkv, row = id / a.Hkv * SA_WAVES + wave;   // (a KV head's rows stay on their chiplet)
     if (row >= a.T * a.G) return;
     const int token = row / a.G, head = hk * a.G + row % a.G;
     const int b = seq_of(a, token);
@@ -592,29 +663,13 @@ __global__ __launch_bounds__(SA_THREADS) void shared_merge_kernel(SharedAttnArgs
     const int64_t rows = (int64_t)a.T * a.Hq, r = (int64_t)token * a.Hq + head;
     constexpr int LPR = D / 4, GROUPS = 64 / LPR;
     const int group = lane / LPR, col = (lane % LPR) * 4;
-    float m_run = -INFINITY, den = 0.f;
+    float m_run, den;
+    start_with_sink<E>(a, head, m_run, den);
     float4_t num = {0.f, 0.f, 0.f, 0.f};
-    if (a.sinks) {   // one more logit in the denominator
-        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
-        m_run = sk != sk ? 0.f : sk;
-        den = sk == -INFINITY ? 0.f : (sk != sk ? sk : 1.0f);
-    }
     for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        const int beg = i < a.np ? i * a.sp : a.prefix_len + (i - a.np) * a.so;
-        const int end = i < a.np ? min(beg + a.sp, a.prefix_len) : beg + a.so;
-        const bool live = i < n && max(beg, lo) < min(end, pos + 1);   // else this row sees none of its keys: nothing was written
-        float m = -INFINITY, l = 0.f;
-        if (live) {
-            m = a.part_ml[(i * rows + r) * 2];
-            l = a.part_ml[(i * rows + r) * 2 + 1];
-        }
-        const float m_new = fmaxf(m_run, wave_max(m));
-        const float back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-        const float f = !live || l == 0.f ? 0.f : (m == m_new ? 1.0f : __builtin_amdgcn_exp2f(m - m_new));
-        den = den * back + wave_sum(f == 0.f && l == l ? 0.f : f * l);
+        float back;
+        const float f = join_stats(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
         num *= back;
-        m_run = m_new;
         const int cnt = min(64, n - i0);
 #pragma unroll 4
         for (int j = group; j < cnt; j += GROUPS) {
@@ -626,95 +681,126 @@ __global__ __launch_bounds__(SA_THREADS) void shared_merge_kernel(SharedAttnArgs
     for (int st = LPR; st < 64; st *= 2)
 #pragma unroll
         for (int c = 0; c < 4; c++) num[c] += __shfl_xor(num[c], st, 64);
-    const float inv = den > 0.f ? 1.0f / den : (den == 0.f ? 0.f : den);   // (a NaN stays one)
+    const float inv = inverse(den);
     if (group == 0) {
         E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + col;
 #pragma unroll
         for (int c = 0; c < 4; c++) out[c] = (E)(num[c] * inv);
     }
-    if (a.final_ml && lane == 0) {
-        a.final_ml[r * 2] = m_run == -INFINITY ? 0.f : m_run;
-        a.final_ml[r * 2 + 1] = inv;
+}
+
+// Adds the own tokens' weights, summed over the group's query heads: a workgroup per (sequence, KV head, SA_SCORE_KEYS
+// tokens), which joins the heads' (m, l) once more for itself instead of waiting for another launch.
+constexpr int SA_SCORE_KEYS = 4 * SA_THREADS;
+template <typename E>
+__device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int pieces) {
+    constexpr int HEADS = 64;
+    __shared__ float fin[HEADS][2];
+    const int hk = id % a.Hkv, piece = id / a.Hkv % pieces, b = id / a.Hkv / pieces, tid = threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ctx = min(a.ctx_lens[b], a.max_ctx), lo = window_lo(a, ctx - 1), first = a.prefix_len + piece * SA_SCORE_KEYS;
+    if (first >= ctx || first + SA_SCORE_KEYS <= lo) return;
+    const int rel = piece * SA_SCORE_KEYS + 4 * tid;
+    float4_t w = {0.f, 0.f, 0.f, 0.f};
+    for (int g0 = 0; g0 < a.G; g0 += HEADS) {
+        const int heads = min(HEADS, a.G - g0);
+        if (g0) __syncthreads();
+        for (int g = wave; g < heads; g += SA_WAVES) {
+            const int head = hk * a.G + g0 + g;
+            float m, den, back;
+            start_with_sink<E>(a, head, m, den);
+            for (int i0 = 0; i0 < a.np + a.ns; i0 += 64) join_stats(range_stat(a, i0 + lane, (int64_t)b * a.Hq + head, ctx - 1, lo), m, den, back);
+            if (lane == 0) {
+                fin[g][0] = m;
+                fin[g][1] = inverse(den);
+            }
+        }
+        __syncthreads();
+        if (a.prefix_len + rel < ctx) {
+            const float* x = a.logits + ((int64_t)b * a.Hq + hk * a.G + g0) * a.lstride + rel;
+#pragma unroll 4
+            for (int g = 0; g < heads; g++) {
+                const float4_t v = *reinterpret_cast<const float4_t*>(x + (int64_t)g * a.lstride);
+#pragma unroll
+                for (int u = 0; u < 4; u++) w[u] += __builtin_amdgcn_exp2f(v[u] - fin[g][0]) * fin[g][1];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int key = a.prefix_len + rel + u;
+        if (key >= ctx || key < lo) continue;
+        const int page = page_of(a, key), blk = a.tables[(int64_t)b * a.max_blocks + page];
+        if (blk < 0 || blk >= a.num_blocks) continue;   // no score is written outside the cache
+        a.scores[((int64_t)blk * a.Hkv + hk) * a.block_size + (key - page * a.block_size)] += w[u];
     }
 }
 
-// Adds the own tokens' weights, summed over the group's query heads: a workgroup per (sequence, KV head, 256 tokens).
-__global__ __launch_bounds__(SA_THREADS) void score_add_kernel(SharedAttnArgs a, int pieces) {
-    const int piece = blockIdx.x % pieces, hk = blockIdx.x / pieces % a.Hkv, b = blockIdx.x / pieces / a.Hkv;
-    const int rel = piece * SA_THREADS + threadIdx.x, key = a.prefix_len + rel;
-    const int ctx = min(a.ctx_lens[b], a.max_ctx);
-    if (key >= ctx || key < window_lo(a, ctx - 1)) return;
-    float w = 0.f;
-    for (int g = 0; g < a.G; g++) {
-        const int64_t r = (int64_t)b * a.Hq + hk * a.G + g;
-        w += __builtin_amdgcn_exp2f(a.logits[r * a.lstride + rel] - a.final_ml[r * 2]) * a.final_ml[r * 2 + 1];
-    }
-    const int page = page_of(a, key), blk = a.tables[(int64_t)b * a.max_blocks + page];
-    if (blk < 0 || blk >= a.num_blocks) return;   // no score is written outside the cache
-    a.scores[((int64_t)blk * a.Hkv + hk) * a.block_size + (key - page * a.block_size)] += w;
+template <typename E, int D>
+__global__ __launch_bounds__(SA_THREADS) void shared_join_kernel(SharedAttnArgs a, int merge_wgs, int pieces) {
+    if ((int)blockIdx.x < merge_wgs) merge_part<E, D>(a, blockIdx.x);
+    else score_part<E>(a, blockIdx.x - merge_wgs, pieces);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// How many ranges a walk over `keys` keys is cut into, for `units` (row set, KV head) pairs: more ranges fill the chip
+// (two workgroups on each of 256 CUs) and even it out, but every range costs a workgroup's start (`start` ns, against `key`
+// ns per key) and `merge` ns of writing and reading its rows' outputs.
+static void cut_keys(int64_t keys, int64_t units, double key, double start, double merge, int& n, int& len) {
+    n = 0, len = 128;
+    double best = 0;
+    for (int64_t c = 1; c <= 1024 && (c == 1 || (c - 1) * 128 < keys); c += c < 16 ? 1 : c / 8) {
+        const int64_t l = ((keys + c - 1) / c + 127) / 128 * 128, used = (keys + l - 1) / l;
+        const double t = (double)((units * used + 511) / 512) * (start + key * l) + merge * used;
+        if (keys > 0 && (n == 0 || t < best)) best = t, n = (int)used, len = (int)l;
+    }
+}
 struct SharedAttnPlan {
     int np, sp, ns, so, lstride;
     int prefix_rows, own_rows;   // rows per workgroup: 32 (RW = 1), 128 or 256 (RW = 4)
-    int64_t units;   // an upper bound of every launch's workgroups and row numbers
+    int64_t units;               // an upper bound of every launch's workgroups and row numbers
     size_t part_floats, logit_floats, bytes;
 };
 static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, bool scored) {
     SharedAttnPlan p;
     max_q = max_q < T ? max_q : T;
-    const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P;
-    p.prefix_rows = T * G <= 32 ? 32 : D == 64 && T * G * Hkv >= 32768 && !scored ? 256 : 128;
+    const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
+    p.prefix_rows = R <= 32 ? 32 : D == 64 && R * Hkv >= 32768 && !scored ? 256 : 128;
     p.own_rows = max_q * G > 32 && !scored ? 128 : 32;
-    // ranges: enough workgroups for the chip, none shorter than 256 keys
-    auto cut = [](int64_t keys, int64_t units, int& n, int& len) {
-        n = 0, len = 256;
-        if (keys <= 0) return;
-        int64_t want = (1024 + units - 1) / units;
-        int64_t l = (keys + want - 1) / want;
-        l = (l + 127) / 128 * 128;
-        if (l < 256) l = 256;
-        len = (int)l;
-        n = (int)((keys + l - 1) / l);
-    };
-    cut(P, (int64_t)Hkv * ((T * G + p.prefix_rows - 1) / p.prefix_rows), p.np, p.sp);
-    cut(own, (int64_t)Hkv * B * ((max_q * G + p.own_rows - 1) / p.own_rows), p.ns, p.so);
+    const double merge = (double)T * Hq * D * 8 / 5000;
+    // a shared tile's keys are paid for in arithmetic, a wave's own tile's in bytes
+    cut_keys(P, Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows), (p.prefix_rows == 32 ? 25.0 : p.prefix_rows == 128 ? 18.0 : 18.0) * D / 64, 3000, merge, p.np, p.sp);
+    cut_keys(own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), (p.own_rows == 32 ? 25.0 : 18.0) * D / 64, 3000, merge, p.ns, p.so);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)((own + 127) / 128 * 128);
-    p.logit_floats = scored ? rows * ((size_t)p.lstride + 2) : 0;
+    p.logit_floats = scored ? rows * (size_t)p.lstride : 0;
     p.bytes = (p.part_floats + p.logit_floats) * sizeof(float);
-    p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_THREADS + 1);
+    p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_SCORE_KEYS + 1);
     return p;
 }
 
 template <typename E, int D>
 static int launch_shared_attn(SharedAttnArgs& a, const SharedAttnPlan& p, bool scored, hipStream_t st) {
-    const int rows = a.T * a.G;
-    if (a.np) {
-        const int grid = a.Hkv * a.np * ((rows + p.prefix_rows - 1) / p.prefix_rows);
-        if (p.prefix_rows == 32 && scored) shared_prefix_kernel<E, D, 1, 1, true><<<grid, SA_THREADS, 0, st>>>(a);
-        else if (p.prefix_rows == 32) shared_prefix_kernel<E, D, 1, 1, false><<<grid, SA_THREADS, 0, st>>>(a);
-        else if (p.prefix_rows == 128 && scored) shared_prefix_kernel<E, D, 4, 1, true><<<grid, SA_THREADS, 0, st>>>(a);
-        else if (p.prefix_rows == 128) shared_prefix_kernel<E, D, 4, 1, false><<<grid, SA_THREADS, 0, st>>>(a);
-        else if constexpr (D == 64) shared_prefix_kernel<E, D, 4, 2, false><<<grid, SA_THREADS, 0, st>>>(a);
-        M355_LAUNCH_CHECK("shared_prefix_kernel");
+    const int rows = a.T * a.G, sets = (a.max_q * a.G + p.own_rows - 1) / p.own_rows;
+    const int np_wgs = a.Hkv * a.np * ((rows + p.prefix_rows - 1) / p.prefix_rows), grid = np_wgs + a.Hkv * a.ns * a.B * sets;
+#define M355_SA(RWP, QT, RWO, SCORED) shared_attn_kernel<E, D, RWP, QT, RWO, SCORED><<<grid, SA_THREADS, 0, st>>>(a, np_wgs, sets)
+    if (grid) {
+        if (scored && p.prefix_rows == 32) M355_SA(1, 1, 1, true);
+        else if (scored) M355_SA(4, 1, 1, true);
+        else if (p.prefix_rows == 32) M355_SA(1, 1, 1, false);
+        else if (p.prefix_rows == 128 && p.own_rows == 32) M355_SA(4, 1, 1, false);
+        else if (p.prefix_rows == 128) M355_SA(4, 1, 4, false);
+        else if constexpr (D == 64) {
+            if (p.own_rows == 32) M355_SA(4, 2, 1, false);
+            else M355_SA(4, 2, 4, false);
+        }
+        M355_LAUNCH_CHECK("shared_attn_kernel");
     }
-    if (a.ns) {
-        const int sets = (a.max_q * a.G + p.own_rows - 1) / p.own_rows, grid = a.Hkv * a.ns * a.B * sets;
-        if (scored) own_tokens_kernel<E, D, 1, true><<<grid, SA_THREADS, 0, st>>>(a, sets);
-        else if (p.own_rows == 128) own_tokens_kernel<E, D, 4, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
-        else own_tokens_kernel<E, D, 1, false><<<grid, SA_THREADS, 0, st>>>(a, sets);
-        M355_LAUNCH_CHECK("own_tokens_kernel");
-    }
-    shared_merge_kernel<E, D><<<a.Hkv * ((rows + SA_WAVES - 1) / SA_WAVES), SA_THREADS, 0, st>>>(a);
-    M355_LAUNCH_CHECK("shared_merge_kernel");
-    if (scored && a.ns) {
-        const int pieces = (a.max_ctx - a.prefix_len + SA_THREADS - 1) / SA_THREADS;
-        score_add_kernel<<<a.Hkv * a.B * pieces, SA_THREADS, 0, st>>>(a, pieces);
-        M355_LAUNCH_CHECK("score_add_kernel");
-    }
+#undef M355_SA
+    const int merge_wgs = a.Hkv * ((rows + SA_WAVES - 1) / SA_WAVES), pieces = scored ? (a.max_ctx - a.prefix_len + SA_SCORE_KEYS - 1) / SA_SCORE_KEYS : 0;
+    shared_join_kernel<E, D><<<merge_wgs + a.Hkv * a.B * pieces, SA_THREADS, 0, st>>>(a, merge_wgs, pieces);
+    M355_LAUNCH_CHECK("shared_join_kernel");
     return 0;
 }
 
@@ -806,7 +892,6 @@ extern "C" int m355_paged_attn_decode_scored(const void* q, const void* kcache, 
         return rc;
     a.logits = a.part_o + p.part_floats;
     a.lstride = p.lstride;
-    a.final_ml = a.logits + (size_t)B * Hq * p.lstride;
     a.scores = scores;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == M355_DTYPE_F16) return D == 64 ? launch_shared_attn<half_t, 64>(a, p, true, st) : launch_shared_attn<half_t, 128>(a, p, true, st);
