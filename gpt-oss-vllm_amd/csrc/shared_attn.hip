@@ -24,11 +24,12 @@ constexpr int SA_THREADS = 256;
 constexpr int SA_WAVES = SA_THREADS / 64;
 constexpr int SA_PAGES = 256;     // entries of a wave's slice of the page table
 constexpr float SA_NONE = -0x1p127f;   // "maximum" of a row that has seen no key: below every score, and finite
-constexpr float SA_LAZY = 6.0f;   // log2 units the running maximum may exceed the exponents' reference point
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef const u32x4_t __attribute__((address_space(3))) sa_lds_u4_t;
 typedef __attribute__((address_space(3))) void sa_lds_void_t;
@@ -146,11 +147,11 @@ __device__ __forceinline__ bool split_nonfinite(u32x4_t v, u32x4_t& clean, u32x4
 template <typename E>
 __device__ __forceinline__ uint32_t pack_p(float p0, float p1, float& sum) {
     if constexpr (__is_same(E, half_t)) {
-        const half2_t ph = {(half_t)p0, (half_t)p1};
+        const half2_t ph = __builtin_convertvector(f32x2_t{p0, p1}, half2_t);
         sum = __builtin_amdgcn_fdot2(ph, half2_t{(half_t)1.0f, (half_t)1.0f}, sum, false);
         return __builtin_bit_cast(uint32_t, ph);
     } else {
-        const bf16x2_t ph = {(bf16_t)p0, (bf16_t)p1};
+        const bf16x2_t ph = __builtin_convertvector(f32x2_t{p0, p1}, bf16x2_t);
         sum = __builtin_amdgcn_fdot2_f32_bf16(ph, bf16x2_t{(bf16_t)1.0f, (bf16_t)1.0f}, sum, false);
         return __builtin_bit_cast(uint32_t, ph);
     }
@@ -231,7 +232,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                                        int split, int own_b, int own_k0) {
     typedef Walk<D, RW> W;
     constexpr int KT = W::KT, ROW = D * 2, STEPS = D / 16, DT = D / 32, NI = W::NI, AHEAD = RW == 1 ? 1 : W::NS - 1;
-    constexpr int VH = RW == 4 && DT == 4 ? 1 : 2;   // V fragments of how many 16-key halves are read ahead of the softmax
+    constexpr int VH = RW == 4 && DT == 4 ? 1 : 2;   // V fragments of how many 16-key halves are held at a time
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 31, hh = lane >> 5;
     int token[QT], head[QT];
@@ -343,8 +344,6 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         }
         // register i of a lane: key k0 + (i & 3) + 8 (i >> 2) + 4 hh
         uint32_t seen[QT];   // (EDGE) bit i: this row sees register i's key
-        float mx[QT];
-        bool move[QT], any = false;
 #pragma unroll
         for (int q = 0; q < QT; q++) {
             if constexpr (EDGE) {
@@ -366,43 +365,53 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                             float4_t{x[q][4 * i4], x[q][4 * i4 + 1], x[q][4 * i4 + 2], x[q][4 * i4 + 3]} * a.scale2;
                 }
             }
-            mx[q] = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) mx[q] = fmaxf(fmaxf(mx[q], x[q][i]), x[q][i + 1]);
-            mx[q] = half_max(fmaxf(mx[q], x[q][15])) * a.scale2;
-            // The exponents' reference follows the running maximum lazily: it moves when a score exceeds it by more than
-            // SA_LAZY, so probabilities reach 2^SA_LAZY instead of 1 (every type holds them, and the denominator carries the
-            // same factor) and the outputs are rescaled a few times per row.
-            move[q] = mx[q] > m_run[q] + SA_LAZY;
-            any |= move[q];
         }
-        if (__any(any)) {
+        // The exponents' reference follows the running maximum lazily: probabilities are formed against the old one, and only
+        // if one of them exceeds 2^12 (seen on the packed 16-bit values, whose order is that of whole numbers) do the maximum,
+        // the rescaling and the probabilities take another turn: a few times per row instead of a maximum per tile.  Every
+        // type holds what lies below, and the denominator carries the same factor.
+        uint32_t pb[QT][8];
+        float sum[QT];
+        auto exponentials = [&] {
+            ushort2_t top = {0, 0};
 #pragma unroll
             for (int q = 0; q < QT; q++) {
-                float alpha = move[q] ? __builtin_amdgcn_exp2f(m_run[q] - mx[q]) : 1.0f;   // (0 for the first key)
-                asm volatile("" : "+v"(alpha));   // (keeps the multiplications below inside this rare branch)
-                if (move[q]) m_run[q] = mx[q];
+                sum[q] = l_run[q];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -m_run[q]));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -m_run[q]));
+                    float rounded = sum[q];
+                    pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
+                    // (the accumulated weights are fp32: their denominator sums the unrounded terms)
+                    sum[q] = SCORED ? sum[q] + (p0 + p1) : rounded;
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, pb[q][i >> 1]));
+                }
+            }
+            return top;
+        };
+        const ushort2_t top = exponentials();
+        constexpr uint16_t LIMIT = __is_same(E, half_t) ? 0x6c00u : 0x4580u;   // 2^12
+        if (__any(top[0] > LIMIT || top[1] > LIMIT)) {
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                float mx = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
+#pragma unroll
+                for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, x[q][i]), x[q][i + 1]);
+                mx = fmaxf(half_max(fmaxf(mx, x[q][15])) * a.scale2, m_run[q]);
+                const float alpha = __builtin_amdgcn_exp2f(m_run[q] - mx);   // (0 for the first key)
+                m_run[q] = mx;
                 l_run[q] *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) o[q][dt][i] *= alpha;
             }
+            exponentials();
         }
-        uint32_t pb[QT][8];
 #pragma unroll
-        for (int q = 0; q < QT; q++) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i], a.scale2, -m_run[q]));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][i + 1], a.scale2, -m_run[q]));
-                float rounded = l_run[q];
-                pb[q][i >> 1] = pack_p<E>(p0, p1, rounded);
-                // (the accumulated weights are fp32: their denominator sums the unrounded terms)
-                l_run[q] = SCORED ? l_run[q] + (p0 + p1) : rounded;
-            }
-        }
-        // element j of step s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
+        for (int q = 0; q < QT; q++) l_run[q] = sum[q];
+        // element j of half s2 is key 16 s2 + 8 (j >> 2) + 4 hh + (j & 3)
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++) {
             if constexpr (VH == 1) {
@@ -602,7 +611,7 @@ __device__ __forceinline__ void own_part(const SharedAttnArgs& a, unsigned char*
 // Both in one launch: the prefix (bound by the matrix cores when there are many rows) and the own tokens (bound by memory)
 // run beside one another.
 template <typename E, int D, int RWP, int QT, int RWO, bool SCORED>
-__global__ __launch_bounds__(SA_THREADS, 2) void shared_attn_kernel(SharedAttnArgs a, int prefix_wgs, int row_sets) {
+__global__ __launch_bounds__(SA_THREADS, D == 64 && QT == 1 ? 3 : 2) void shared_attn_kernel(SharedAttnArgs a, int prefix_wgs, int row_sets) {
     constexpr int LP = Walk<D, RWP>::LDS, LO = Walk<D, RWO>::LDS;
     __shared__ __attribute__((aligned(16))) unsigned char smem[LP > LO ? LP : LO];
     if ((int)blockIdx.x < prefix_wgs) prefix_part<E, D, RWP, QT, SCORED>(a, smem, blockIdx.x);
@@ -636,57 +645,66 @@ __device__ __forceinline__ void start_with_sink(const SharedAttnArgs& a, int hea
         den = sk == -INFINITY ? 0.f : sk == sk ? 1.0f : sk;   // (a NaN stays one)
     }
 }
-// One 64 ranges' step of the running (m, den): returns this lane's factor (0: leave its range out).
+// One step of the running (m, den) over the ranges of N neighbouring lanes: returns this lane's factor (0: leave its range
+// out).
+template <int N>
 __device__ __forceinline__ float join_stats(const RangeStat& s, float& m_run, float& den, float& back) {
-    const float m_new = fmaxf(m_run, wave_max(s.m));
+    float top = s.m;
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float m_new = fmaxf(m_run, top);
     back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
     const float f = !s.live || s.l == 0.f ? 0.f : s.m == m_new ? 1.0f : __builtin_amdgcn_exp2f(s.m - m_new);
-    den = den * back + wave_sum(f == 0.f && s.l == s.l ? 0.f : f * s.l);
+    float part = f == 0.f && s.l == s.l ? 0.f : f * s.l;
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) part += __shfl_xor(part, o, 64);
+    den = den * back + part;
     m_run = m_new;
     return f;
 }
 __device__ __forceinline__ float inverse(float den) { return den > 0.f ? 1.0f / den : den == 0.f ? 0.f : den; }
 
-// Joins a row's ranges: a wave per (token, query head).  A lane looks after one range's (m, l), then the lanes stand D / 4 to
-// a range's row and 64 / (D / 4) ranges go by at a time.
-template <typename E, int D>
+// Joins a row's ranges, LANES lanes per (token, query head): each looks after one range's (m, l), then they take the ranges'
+// outputs on, D / 4 lanes to a range's row.  LANES = 64: a wave's whole width on one row, LANES / (D / 4) ranges at a time,
+// for few rows with many ranges.  LANES = D / 4: several rows per wave, for many rows (waves beyond what the chip holds at
+// once cost another round of memory latency: 109000 rows of 3 ranges took 57 us a wave each, 20 us this way, and 2048 rows of
+// 34 ranges 6 us and 14).
+template <typename E, int D, int LANES>
 __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = id % a.Hkv, row = id / a.Hkv * SA_WAVES + wave;   // (a KV head's rows stay on their chiplet)
-    if (row >= a.T * a.G) return;
+    constexpr int LPR = D / 4, GROUPS = LANES / LPR, ROWS = SA_THREADS / LANES;
+    const int lane = threadIdx.x % LANES, base = (threadIdx.x & 63) - lane, group = lane / LPR, col = lane % LPR * 4;
+    const int hk = id % a.Hkv, row_asked = id / a.Hkv * ROWS + (int)threadIdx.x / LANES;   // (a KV head's rows stay on their chiplet)
+    const int row = min(row_asked, a.T * a.G - 1);
     const int token = row / a.G, head = hk * a.G + row % a.G;
     const int b = seq_of(a, token);
-    if (b < 0) return;   // behind the last sequence: left as it was
-    const SeqSpan s = seq_span(a, b);
-    if (token - s.t0 >= a.max_q) return;
+    const SeqSpan s = seq_span(a, max(b, 0));
     const int pos = s.ctx - s.n + (token - s.t0), lo = window_lo(a, pos), n = a.np + a.ns;
     const int64_t rows = (int64_t)a.T * a.Hq, r = (int64_t)token * a.Hq + head;
-    constexpr int LPR = D / 4, GROUPS = 64 / LPR;
-    const int group = lane / LPR, col = (lane % LPR) * 4;
     float m_run, den;
     start_with_sink<E>(a, head, m_run, den);
     float4_t num = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < n; i0 += 64) {
+    for (int i0 = 0; i0 < n; i0 += LANES) {   // (every lane of the wave goes along: the sums below span its rows' lanes)
         float back;
-        const float f = join_stats(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
+        const float f = join_stats<LANES>(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
         num *= back;
-        const int cnt = min(64, n - i0);
+        const int cnt = min(LANES, n - i0);
 #pragma unroll 4
         for (int j = group; j < cnt; j += GROUPS) {
-            const float fj = __shfl(f, j, 64);
-            if (fj != 0.f) num += fj * *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
+            const float fj = __shfl(f, base + j, 64);
+            const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
+            if (fj != 0.f) num += fj * v;   // (what was not written may be anything)
         }
     }
 #pragma unroll
-    for (int st = LPR; st < 64; st *= 2)
+    for (int st = LPR; st < LANES; st *= 2)
 #pragma unroll
         for (int c = 0; c < 4; c++) num[c] += __shfl_xor(num[c], st, 64);
+    // rows behind the last sequence, and tokens behind the longest one that was announced, leave the output as it was
+    if (group || row_asked >= a.T * a.G || b < 0 || token - s.t0 >= a.max_q) return;
     const float inv = inverse(den);
-    if (group == 0) {
-        E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + col;
+    E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + col;
 #pragma unroll
-        for (int c = 0; c < 4; c++) out[c] = (E)(num[c] * inv);
-    }
+    for (int c = 0; c < 4; c++) out[c] = (E)(num[c] * inv);
 }
 
 // Adds the own tokens' weights, summed over the group's query heads: a workgroup per (sequence, KV head, SA_SCORE_KEYS
@@ -709,7 +727,7 @@ __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int 
             const int head = hk * a.G + g0 + g;
             float m, den, back;
             start_with_sink<E>(a, head, m, den);
-            for (int i0 = 0; i0 < a.np + a.ns; i0 += 64) join_stats(range_stat(a, i0 + lane, (int64_t)b * a.Hq + head, ctx - 1, lo), m, den, back);
+            for (int i0 = 0; i0 < a.np + a.ns; i0 += 64) join_stats<64>(range_stat(a, i0 + lane, (int64_t)b * a.Hq + head, ctx - 1, lo), m, den, back);
             if (lane == 0) {
                 fin[g][0] = m;
                 fin[g][1] = inverse(den);
@@ -736,9 +754,9 @@ __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int 
     }
 }
 
-template <typename E, int D>
+template <typename E, int D, int LANES>
 __global__ __launch_bounds__(SA_THREADS) void shared_join_kernel(SharedAttnArgs a, int merge_wgs, int pieces) {
-    if ((int)blockIdx.x < merge_wgs) merge_part<E, D>(a, blockIdx.x);
+    if ((int)blockIdx.x < merge_wgs) merge_part<E, D, LANES>(a, blockIdx.x);
     else score_part<E>(a, blockIdx.x - merge_wgs, pieces);
 }
 
@@ -798,8 +816,11 @@ static int launch_shared_attn(SharedAttnArgs& a, const SharedAttnPlan& p, bool s
         M355_LAUNCH_CHECK("shared_attn_kernel");
     }
 #undef M355_SA
-    const int merge_wgs = a.Hkv * ((rows + SA_WAVES - 1) / SA_WAVES), pieces = scored ? (a.max_ctx - a.prefix_len + SA_SCORE_KEYS - 1) / SA_SCORE_KEYS : 0;
-    shared_join_kernel<E, D><<<merge_wgs + a.Hkv * a.B * pieces, SA_THREADS, 0, st>>>(a, merge_wgs, pieces);
+    const bool many = (int64_t)rows * a.Hkv > 16384;   // twice the waves that the chip holds at once
+    const int per = SA_THREADS / (many ? D / 4 : 64), merge_wgs = a.Hkv * ((rows + per - 1) / per);
+    const int pieces = scored ? (a.max_ctx - a.prefix_len + SA_SCORE_KEYS - 1) / SA_SCORE_KEYS : 0, join_grid = merge_wgs + a.Hkv * a.B * pieces;
+    if (many) shared_join_kernel<E, D, D / 4><<<join_grid, SA_THREADS, 0, st>>>(a, merge_wgs, pieces);
+    else shared_join_kernel<E, D, 64><<<join_grid, SA_THREADS, 0, st>>>(a, merge_wgs, pieces);
     M355_LAUNCH_CHECK("shared_join_kernel");
     return 0;
 }
