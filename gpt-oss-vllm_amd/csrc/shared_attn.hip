@@ -483,35 +483,46 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         t = tiles_of_kind(std::false_type{}, t);
     }
 
+    // The outputs go through LDS (in place of the tiles), so that whole rows are stored: straight from the accumulators a
+    // store would touch 32 rows with 32 bytes each.  16-byte chunk c of row r lies at chunk c ^ (r & 15).
     const int64_t rows = (int64_t)a.T * a.Hq;
-    if constexpr (RW == 4) {
-#pragma unroll
-        for (int q = 0; q < QT; q++) {
-            const float l = half_sum(l_run[q]);
-            if (mine[q]) {
-                const int64_t r = split * rows + (int64_t)token[q] * a.Hq + head[q];
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; i4++)
-                        *reinterpret_cast<float4_t*>(a.part_o + r * D + 32 * dt + 8 * i4 + 4 * hh) =
-                            float4_t{o[q][dt][4 * i4], o[q][dt][4 * i4 + 1], o[q][dt][4 * i4 + 2], o[q][dt][4 * i4 + 3]};
-                if (hh == 0) {
-                    a.part_ml[r * 2] = m_run[q];
-                    a.part_ml[r * 2 + 1] = l;
-                }
-            }
-        }
-    } else {
-        static_assert(QT == 1 && 32 * D * 4 <= W::STAGE);
-        __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
-        auto po = [&](int w, int r) { return reinterpret_cast<float*>(smem + w * W::NS * W::STAGE) + r * D; };   // in place of the wave's tiles
+    constexpr int CH = D / 4;   // 16-byte chunks, and lanes, per row
+    auto put = [&](unsigned char* at, const f32x16_t(&acc)[DT]) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++)
-                *reinterpret_cast<float4_t*>(po(wave, qi) + 32 * dt + 8 * i4 + 4 * hh) =
-                    float4_t{o[0][dt][4 * i4], o[0][dt][4 * i4 + 1], o[0][dt][4 * i4 + 2], o[0][dt][4 * i4 + 3]};
+                *reinterpret_cast<float4_t*>(at + qi * D * 4 + (((8 * dt + 2 * i4 + hh) ^ (qi & 15)) << 4)) =
+                    float4_t{acc[dt][4 * i4], acc[dt][4 * i4 + 1], acc[dt][4 * i4 + 2], acc[dt][4 * i4 + 3]};
+    };
+    auto get = [&](const unsigned char* at, int r, int c) { return *reinterpret_cast<const float4_t*>(at + r * D * 4 + ((c ^ (r & 15)) << 4)); };
+    if constexpr (RW == 4) {
+        static_assert(SA_WAVES * 32 * D * 4 <= W::TILES);
+        unsigned char* at = smem + wave * 32 * D * 4;
+        __syncthreads();   // every wave is done with the tiles
+#pragma unroll
+        for (int q = 0; q < QT; q++) {
+            put(at, o[q]);
+            const float l = half_sum(l_run[q]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const int first = row0 + 32 * (wave * QT + q), c = lane % CH;
+#pragma unroll
+            for (int i = 0; i < 32 * CH / 64; i++) {
+                const int r32 = i * (64 / CH) + lane / CH, rr = first + r32;
+                const float4_t v = get(at, r32, c);
+                if (rr < row_end) *reinterpret_cast<float4_t*>(a.part_o + (split * rows + (int64_t)(rr / a.G) * a.Hq + hk * a.G + rr % a.G) * D + 4 * c) = v;
+            }
+            if (mine[q] && hh == 0) {
+                const int64_t r = split * rows + (int64_t)token[q] * a.Hq + head[q];
+                a.part_ml[r * 2] = m_run[q];
+                a.part_ml[r * 2 + 1] = l;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    } else {
+        static_assert(QT == 1 && 32 * D * 4 <= W::STAGE);
+        __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
+        put(tiles, o[0]);   // (each wave in place of its own tile)
         const float lsum = half_sum(l_run[0]);
         if (hh == 0) {
             wm[wave][qi] = m_run[0];
@@ -519,8 +530,8 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         }
         __syncthreads();
         const int nrows = min(32, row_end - row0);
-        for (int i = tid; i < nrows * (D / 4); i += SA_THREADS) {
-            const int r32 = i / (D / 4), d = (i % (D / 4)) * 4;
+        for (int i = tid; i < nrows * CH; i += SA_THREADS) {
+            const int r32 = i / CH, c = i % CH;
             float m = wm[0][r32];
 #pragma unroll
             for (int w = 1; w < SA_WAVES; w++) m = fmaxf(m, wm[w][r32]);
@@ -529,13 +540,13 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 #pragma unroll
             for (int w = 0; w < SA_WAVES; w++) {
                 const float f = wm[w][r32] == m ? 1.0f : __builtin_amdgcn_exp2f(wm[w][r32] - m);   // (nothing seen at all: 1 * 0)
-                tot += f * *reinterpret_cast<const float4_t*>(po(w, r32) + d);
+                tot += f * get(smem + w * W::NS * W::STAGE, r32, c);
                 l += f * wl[w][r32];
             }
             const int rr = row0 + r32;
             const int64_t r = split * rows + (int64_t)(rr / a.G) * a.Hq + hk * a.G + rr % a.G;
-            *reinterpret_cast<float4_t*>(a.part_o + r * D + d) = tot;
-            if (d == 0) {
+            *reinterpret_cast<float4_t*>(a.part_o + r * D + 4 * c) = tot;
+            if (c == 0) {
                 a.part_ml[r * 2] = m;
                 a.part_ml[r * 2 + 1] = l;
             }
