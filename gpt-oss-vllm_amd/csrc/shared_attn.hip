@@ -16,6 +16,7 @@
 //                            operands; o and l stay fp32), are the B operand; V^T comes from LDS through the transposing read.
 #include "common.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace m355 {
@@ -772,16 +773,24 @@ __global__ __launch_bounds__(SA_THREADS) void shared_join_kernel(SharedAttnArgs 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// How many ranges a walk over `keys` keys is cut into, for `units` (row set, KV head) pairs: more ranges fill the chip
-// (two workgroups on each of 256 CUs) and even it out, but every range costs a workgroup's start (`start` ns, against `key`
-// ns per key) and `merge` ns of writing and reading its rows' outputs.
-static void cut_keys(int64_t keys, int64_t units, double key, double start, double merge, int& n, int& len) {
+// Into how many ranges a walk over `keys` keys is cut, for `units` (row set, KV head) pairs.  More ranges fill the 256 CUs
+// and even them out; each costs its workgroups' start and the writing and reading of its rows' outputs.  In ns, fitted to
+// sweeps of 1 to 64 ranges over prefixes of 8192 and 20011 keys, 32 to 2500 tokens, and own contexts of 512 to 65536:
+//   7000 + len * max(alone, share * c) + 1300 c + merge * n     c: workgroups per CU, whole ones until there are four
+// alone: ns per key of one workgroup on a CU, share: of all of a CU's workgroups together.  A few workgroups over a whole
+// number per CU cost arithmetic (`tiles`) little, memory another round.  `beside`: time of memory-bound work of the same
+// launch, which runs in the shadow of one workgroup per CU, but behind a second one.
+static void cut_keys(int64_t keys, int64_t units, bool tiles, double alone, double share, double merge, double beside, int& n, int& len) {
     n = 0, len = 128;
+    if (keys <= 0) return;
     double best = 0;
-    for (int64_t c = 1; c <= 1024 && (c == 1 || (c - 1) * 128 < keys); c += c < 16 ? 1 : c / 8) {
-        const int64_t l = ((keys + c - 1) / c + 127) / 128 * 128, used = (keys + l - 1) / l;
-        const double t = (double)((units * used + 511) / 512) * (start + key * l) + merge * used;
-        if (keys > 0 && (n == 0 || t < best)) best = t, n = (int)used, len = (int)l;
+    for (int64_t k = 1; k <= 1024 && (k == 1 || (k - 1) * 128 < keys); k += k < 16 ? 1 : k / 8) {
+        const int64_t l = ((keys + k - 1) / k + 127) / 128 * 128, used = (keys + l - 1) / l;
+        const double c = (double)(units * used) / 256, whole = c <= 1 ? 1 : c < 4 ? ceil(c - (tiles ? 0.125 : 0)) : c;
+        const double per_key = share * whole;
+        const double behind = c <= 1 ? 0 : c < 2 ? c - 1 : 1;
+        const double t = 7000 + l * (per_key > alone ? per_key : alone) + 1300 * c + merge * used + 0.5 * behind * beside;
+        if (n == 0 || t < best) best = t, n = (int)used, len = (int)l;
     }
 }
 struct SharedAttnPlan {
@@ -796,10 +805,15 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
     p.prefix_rows = R <= 32 ? 32 : D == 64 && R * Hkv >= 32768 && !scored ? 256 : 128;
     p.own_rows = max_q * G > 32 && !scored ? 128 : 32;
-    const double merge = (double)T * Hq * D * 8 / 5000;
-    // a shared tile's keys are paid for in arithmetic, a wave's own tile's in bytes
-    cut_keys(P, Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows), (p.prefix_rows == 32 ? 25.0 : p.prefix_rows == 128 ? 18.0 : 18.0) * D / 64, 3000, merge, p.np, p.sp);
-    cut_keys(own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), (p.own_rows == 32 ? 25.0 : 18.0) * D / 64, 3000, merge, p.ns, p.so);
+    const double merge = (double)T * Hq * D * 4 / 2500, wide = D / 64;
+    auto cut = [&](int64_t keys, int64_t units, int rows, double beside, int& n, int& len) {
+        if (rows == 32) cut_keys(keys, units, false, 14 * wide, 13 * wide, merge, beside, n, len);
+        else if (rows == 128) cut_keys(keys, units, true, wide == 1 ? 18 : 33, wide == 1 ? 11.2 : 20, merge, beside, n, len);
+        else cut_keys(keys, units, true, 36, 21.7, merge, beside, n, len);
+    };
+    cut(P, Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows), p.prefix_rows,
+        p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0, p.np, p.sp);
+    cut(own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), p.own_rows, 0, p.ns, p.so);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)((own + 127) / 128 * 128);
