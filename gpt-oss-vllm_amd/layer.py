@@ -72,6 +72,43 @@ def validate_paging(block_tables: torch.Tensor, slots: torch.Tensor, ctx_lens: t
         raise ValueError(f"slot {int(sl.max())} outside the cache of {nblocks * block_size} rows")
 
 
+def validate_eviction(block_tables: torch.Tensor, ctx_lens: torch.Tensor, dst_tables: torch.Tensor, kcache: torch.Tensor, *, keep: int,
+                      prefix_len: int = 0) -> None:
+    """Host-side check (synchronises) of what kv_evict trusts: the pages that will receive kept tokens lie inside the cache,
+    are handed out once, and are none of those that the call reads.  Meant to run where the pages are handed out."""
+    nblocks, block_size = kcache.shape[0], kcache.shape[1]
+    src, dst = block_tables.detach().cpu(), dst_tables.detach().cpu()
+    first, seen = prefix_len // block_size, set()
+    read = set()
+    for b, ctx in enumerate(ctx_lens.detach().cpu().tolist()):
+        read.update(src[b if ctx > prefix_len else 0, :(ctx + block_size - 1) // block_size].tolist())
+    read.update(src[0, :first].tolist())
+    for b, ctx in enumerate(ctx_lens.detach().cpu().tolist()):
+        end = prefix_len + min(max(ctx - prefix_len, 0), keep)
+        need = (end + block_size - 1) // block_size
+        if need > dst.shape[1]:
+            raise ValueError(f"sequence {b} keeps {end} tokens in {need} pages, dst_tables holds {dst.shape[1]}")
+        for page in dst[b, first:need].tolist():
+            if page < 0 or page >= nblocks:
+                raise ValueError(f"sequence {b}: destination page {page} outside [0, {nblocks})")
+            if page in seen or page in read:
+                raise ValueError(f"sequence {b}: destination page {page} is in use")
+            seen.add(page)
+
+
+def evict_tokens(caches, scores, block_tables: torch.Tensor, ctx_lens: torch.Tensor, dst_tables: torch.Tensor, *, keep: int, recent: int,
+                 max_ctx: int, prefix_len: int = 0, new_lens=None) -> torch.Tensor:
+    """Trim every layer's cache by its own scores: caches [(kcache, vcache)] and scores [blocks][Hkv][block_size] per layer,
+    tables and lengths shared by the layers.  Layers and heads keep different tokens but equally many, in order, so the new
+    tables and lengths (returned) serve them all; `recent` of at least a sliding window leaves windowed layers unharmed.
+    Rotary positions go on counting from the old lengths: keys were rotated when they were written."""
+    from . import lib
+    for (kc, vc), sc in zip(caches, scores):
+        _, new_lens = lib.kv_evict(kc, vc, sc, block_tables, ctx_lens, dst_tables, keep=keep, recent=recent, max_ctx=max_ctx,
+                                   prefix_len=prefix_len, new_lens=new_lens)
+    return new_lens
+
+
 # ---------------------------------------------------------------------------------------------
 # One gpt-oss decoder layer at decode time, as a fixed sequence of library calls on preallocated buffers
 # ---------------------------------------------------------------------------------------------
@@ -135,25 +172,35 @@ class GptOssDecodeLayer:
         qkv = lib.linear_f16(h, w["wqkv"], w.get("bqkv"))
         lib.rope_kv_write(qkv, cos, sin, positions, slots, kcache, vcache, Hq=self.Hq, Hkv=self.Hkv, D=self.D)
 
-    def prefill(self, resid_in, delta, positions, slots, seq_starts, max_seq: int, kcache, vcache, cos, sin):
+    def prefill(self, resid_in, delta, positions, slots, seq_starts, max_seq: int, kcache, vcache, cos, sin, *, block_tables=None,
+                ctx_lens=None, max_ctx: int = 0, prefix_len: int = 0):
         """The same layer over whole prompts: resid_in [tokens][H] holds the sequences one after another, seq_starts
         int32 [B + 1] their first rows, positions the rotary positions, slots the cache rows of the tokens (negative:
         not cached).  Attention is causal within each sequence (m355_attn_prefill) over the rotated keys of this
-        call, so the sequences must start at position 0 of their context.  Buffers are allocated per call (prompt
-        sizes vary).  Returns (residual stream after attention, expert output), as forward does."""
+        call, so the sequences must start at position 0 of their context -- unless block_tables [B][max_blocks], ctx_lens
+        [B] (these tokens counted) and max_ctx are given: then the tokens continue what the cache already holds, of which
+        the first prefix_len tokens are shared by all sequences (m355_shared_prefix_attn), and every token needs a slot.
+        Buffers are allocated per call (prompt sizes vary).  Returns (residual stream after attention, expert output), as
+        forward does."""
         lib, w = self.lib, self.w
         T, dev = resid_in.shape[0], resid_in.device
         resid = torch.empty_like(resid_in)
         h1 = lib.add_rmsnorm(resid_in, delta, w["ln1"], self.eps, resid_out=resid)
         qkv = lib.linear_f16(h1, w["wqkv"], w.get("bqkv"))
-        # rotated keys and the values of the prompt, token-major, for the attention; then the same rows into the cache
-        k_rows = torch.empty((T, 1, self.Hkv, self.D), dtype=torch.float16, device=dev)
-        v_rows = torch.empty_like(k_rows)
-        q = lib.rope_kv_write(qkv, cos, sin, positions, torch.arange(T, dtype=torch.int64, device=dev), k_rows, v_rows,
-                              Hq=self.Hq, Hkv=self.Hkv, D=self.D)
-        lib.rope_kv_write(qkv, cos, sin, positions, slots, kcache, vcache, Hq=self.Hq, Hkv=self.Hkv, D=self.D, q_out=q)
-        attn = lib.attn_prefill(q, k_rows.view(T, self.Hkv, self.D), v_rows.view(T, self.Hkv, self.D), seq_starts, max_seq,
-                                scale=self.D ** -0.5, sinks=w.get("sinks"), window=self.window)
+        if block_tables is not None:
+            q = lib.rope_kv_write(qkv, cos, sin, positions, slots, kcache, vcache, Hq=self.Hq, Hkv=self.Hkv, D=self.D)
+            attn = lib.shared_prefix_attn(q, kcache, vcache, block_tables, ctx_lens, prefix_len=prefix_len, max_ctx=max_ctx,
+                                          scale=self.D ** -0.5, seq_starts=seq_starts, max_q=max_seq, sinks=w.get("sinks"),
+                                          window=self.window)
+        else:
+            # rotated keys and the values of the prompt, token-major, for the attention; then the same rows into the cache
+            k_rows = torch.empty((T, 1, self.Hkv, self.D), dtype=torch.float16, device=dev)
+            v_rows = torch.empty_like(k_rows)
+            q = lib.rope_kv_write(qkv, cos, sin, positions, torch.arange(T, dtype=torch.int64, device=dev), k_rows, v_rows,
+                                  Hq=self.Hq, Hkv=self.Hkv, D=self.D)
+            lib.rope_kv_write(qkv, cos, sin, positions, slots, kcache, vcache, Hq=self.Hq, Hkv=self.Hkv, D=self.D, q_out=q)
+            attn = lib.attn_prefill(q, k_rows.view(T, self.Hkv, self.D), v_rows.view(T, self.Hkv, self.D), seq_starts, max_seq,
+                                    scale=self.D ** -0.5, sinks=w.get("sinks"), window=self.window)
         resid2 = lib.linear_f16(attn.view(T, self.Hq * self.D), w["wo"], w.get("bo"), resid=resid)
         h2 = lib.add_rmsnorm(resid2, None, w["ln2"], self.eps)
         moe_out, _, _ = lib.moe_nf4_forward_routed(h2, w["router_w"], w.get("router_b"), self.k, w["w13_q"], w["w13_absmax"],
@@ -162,13 +209,15 @@ class GptOssDecodeLayer:
         return resid2, moe_out
 
     def forward(self, resid_in, delta, positions, slots, block_tables, ctx_lens, kcache, vcache, cos, sin, max_ctx: int,
-                defer_combine: bool = False):
+                defer_combine: bool = False, prefix_len: int = 0, scores=None):
         """resid_in [T][H]: the residual stream entering the layer, delta: the previous layer's expert output still to
         be added (None for the first layer; a PendingCombine when that layer ran with defer_combine).  ctx_lens counts
         the new token.  Returns (residual stream after attention, expert output): their sum is the layer's output.
         defer_combine: the expert output is returned as a PendingCombine (the experts' rows still unsummed in this
         layer's workspace); the next layer's first kernel then forms it together with the residual add and its
-        RMSNorm, one launch less per layer, same bits."""
+        RMSNorm, one launch less per layer, same bits.
+        prefix_len: the first tokens of every sequence are the same, read through row 0 of block_tables once for all.
+        scores [blocks][Hkv][block_size] fp32: every own token's attention weight is added there, for evict_tokens."""
         lib, w = self.lib, self.w
         T = resid_in.shape[0]
         if T != self.T:
@@ -179,11 +228,21 @@ class GptOssDecodeLayer:
         lib.norm_qkv_rope_kv_write(resid_in, pending, w["ln1"], self.eps, w["wqkv"], w.get("bqkv"), cos, sin, positions, slots,
                                    kcache, vcache, Hq=self.Hq, Hkv=self.Hkv, D=self.D, resid_out=self.resid, q_out=self.q,
                                    h_scratch=self.h1, qkv_scratch=self.qkv)
-        need = lib.paged_attn_workspace_bytes(T, self.Hq, self.D, max_ctx)
+        if scores is not None:
+            need = lib.paged_attn_decode_scored_workspace_bytes(T, self.Hq, self.Hkv, self.D, max_ctx, prefix_len)
+        elif prefix_len:
+            need = lib.shared_prefix_attn_workspace_bytes(T, T, 1, self.Hq, self.Hkv, self.D, max_ctx, prefix_len)
+        else:
+            need = lib.paged_attn_workspace_bytes(T, self.Hq, self.D, max_ctx)
         if need and (self.attn_ws is None or self.attn_ws.numel() < need):
             self.attn_ws = torch.empty(need, dtype=torch.uint8, device=self.q.device)
-        lib.paged_attn_decode(self.q, kcache, vcache, block_tables, ctx_lens, max_ctx=max_ctx, scale=self.D ** -0.5,
-                              workspace=self.attn_ws, out=self.attn, sinks=w.get("sinks"), window=self.window)
+        attn_args = dict(max_ctx=max_ctx, scale=self.D ** -0.5, workspace=self.attn_ws, out=self.attn, sinks=w.get("sinks"), window=self.window)
+        if scores is not None:
+            lib.paged_attn_decode_scored(self.q, kcache, vcache, scores, block_tables, ctx_lens, prefix_len=prefix_len, **attn_args)
+        elif prefix_len:
+            lib.shared_prefix_attn(self.q, kcache, vcache, block_tables, ctx_lens, prefix_len=prefix_len, **attn_args)
+        else:
+            lib.paged_attn_decode(self.q, kcache, vcache, block_tables, ctx_lens, **attn_args)
         lib.linear_f16(self.attn.view(T, self.Hq * self.D), w["wo"], w.get("bo"), resid=self.resid, out=self.resid2)
         # the router rides in the launch of the norm in front of the MoE block (one workgroup per token has the normalised
         # row at hand).  Measured against the norm alone followed by m355_moe_nf4_forward_routed (logits as a launch of

@@ -379,3 +379,213 @@ def test_wrappers_refuse_cpu_tensors(m355):
         m355.paged_attn_decode_scored(q, c.k, c.v, c.scores, c.tables, cl, max_ctx=32, scale=0.1)
     with pytest.raises(m355.Mi355LibraryError, match="GPU tensor"):
         m355.kv_evict(c.k, c.v, c.scores, c.tables, cl, c.dst, keep=16, recent=1, max_ctx=32)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the three together, through the decoder layer
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,P", [("full", 112), ("full", 117), ("sliding", 112), ("sliding", 150)])
+def test_gpu_layer_serves_sequences_on_a_shared_prefix(name, P, m355, cuda):
+    """A 201-token text whose first P tokens are cached once: three sequences continue it with prompts of different lengths
+    (packed, one pass over the shared pages), then take the next token in a decode step; every row against transformers'
+    decoder layer.  The decode step adds up the tokens' weights, the caches are trimmed, and another step on the trimmed
+    cache equals the formula over the kept tokens."""
+    from gpt_oss_vllm_amd import layer
+    from test_layer_ops import _decoder_layer, _g
+    B, bs, S = 3, 16, 201
+    lyr, p = _decoder_layer(name, B)
+    Hkv, D = p["Hkv"], p["D"]
+    want = _g(f"layer_decoder_rows.{name}.npy")
+    x = torch.from_numpy(p["x"]).to(cuda)
+    pages = (S + 3 + bs - 1) // bs
+    first = P // bs
+    n = (pages - first) * (2 * B) + pages + 2
+    ids = torch.randperm(n, generator=torch.Generator().manual_seed(P)).tolist()
+    shared = [ids.pop() for _ in range(pages)]
+    tables = [shared] + [shared[:first] + [ids.pop() for _ in range(pages - first)] for _ in range(B - 1)]
+    bt = torch.tensor(tables, dtype=torch.int32, device=cuda)
+    # (pages that nobody has written hold NaN)
+    kc = torch.full((n, bs, Hkv, D), float("nan"), dtype=F16, device=cuda)
+    vc = torch.full_like(kc, float("nan"))
+    cos, sin = (t.to(cuda) for t in layer.rope_tables(512))
+    slot = lambda b, t: tables[0 if t < P else b][t // bs] * bs + t % bs      # noqa: E731
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)           # noqa: E731
+    i64 = lambda v: torch.tensor(v, dtype=torch.int64, device=cuda)           # noqa: E731
+    # the shared tokens, once
+    r, m = lyr.prefill(x[:P].contiguous(), None, i32(range(P)), i64([slot(0, t) for t in range(P)]), i32([0, P]), P, kc, vc, cos, sin)
+    tol = 5e-3 * np.abs(want).max()
+    assert np.abs((r.float() + m.float()).cpu().numpy() - want[:P]).max() <= tol
+    # the sequences' own prompts: up to 200, 171 and 160 tokens of the text
+    ends = [200, 171, 160]
+    toks = [(b, t) for b in range(B) for t in range(P, ends[b])]
+    starts = np.concatenate([[0], np.cumsum([e - P for e in ends])])
+    r, m = lyr.prefill(torch.stack([x[t] for _, t in toks]), None, i32([t for _, t in toks]), i64([slot(b, t) for b, t in toks]), i32(starts),
+                       max(ends) - P, kc, vc, cos, sin, block_tables=bt, ctx_lens=i32(ends), max_ctx=max(ends), prefix_len=P)
+    got = (r.float() + m.float()).cpu().numpy()
+    assert np.abs(got - want[[t for _, t in toks]]).max() <= tol
+    # the next token of each, twice over the same cache: without and with the weights added up
+    step = lambda pos, where, tb, ctx, **kw: lyr.forward(torch.stack([x[t] for t in ends]), None, i32(pos), i64(where), tb, i32(ctx), kc, vc,  # noqa: E731
+                                                         cos, sin, max_ctx=tb.shape[1] * bs, **kw)
+    scores = torch.zeros((n, Hkv, bs), device=cuda)
+    where = [slot(b, e) for b, e in enumerate(ends)]
+    outs = []
+    for sc in (None, scores):
+        r, m = step(ends, where, bt, [e + 1 for e in ends], prefix_len=P, scores=sc)
+        outs.append((r.float() + m.float()).cpu().numpy())
+        assert np.abs(outs[-1] - want[ends]).max() <= tol
+    # the weights of a KV head's queries add up to their number, less what the prefix and the sinks took
+    total = torch.stack([scores[bt[b].long()].sum(dim=(0, 2)) for b in range(B)]).cpu()
+    assert (total > 0).all() and (total < p["Hq"] // Hkv * (1 + 1e-5)).all()
+    if P % bs:
+        with pytest.raises(m355.Mi355LibraryError, match="multiple of block_size"):
+            layer.evict_tokens([(kc, vc)], [scores], bt, i32([e + 1 for e in ends]), bt, keep=20, recent=5, max_ctx=S, prefix_len=P)
+        return
+    # trim: of every sequence's own tokens 20 remain, 5 of them the last
+    keep, recent = 20, 5
+    dst = [shared[:first] + [ids.pop() for _ in range((keep + 1 + bs - 1) // bs)] for _ in range(B)]
+    dt = i32(dst)
+    ctx = i32([e + 1 for e in ends])
+    layer.validate_eviction(bt, ctx, dt, kc, keep=keep, prefix_len=P)
+    with pytest.raises(ValueError, match="in use"):
+        layer.validate_eviction(bt, ctx, bt, kc, keep=keep, prefix_len=P)
+    c = Cache.__new__(Cache)                     # the oracle's view of the cache before the call
+    c.ctx, c.prefix, c.block, c.Hkv, c.scores, c.tables = [e + 1 for e in ends], P, bs, Hkv, scores.cpu().clone(), bt.cpu()
+    kept, lens = evict_oracle(c, keep, recent)
+    kept_d, lens_d = m355.kv_evict(kc, vc, scores, bt, ctx, dt, keep=keep, recent=recent, max_ctx=S, prefix_len=P)
+    assert torch.equal(kept_d.cpu(), kept) and lens_d.tolist() == lens == [P + keep] * B
+    # the step after that: positions go on, slots follow the trimmed lengths.  Against the same layer's formula: the
+    # attention over the kept rows in 64 bits on the layer's own q, then the layer's projection
+    where = [dst[b][(P + keep) // bs] * bs + (P + keep) % bs for b in range(B)]
+    before = scores.clone()
+    step([e + 1 for e in ends], where, dt, [P + keep + 1] * B, prefix_len=P, scores=scores)
+    c.ctx, c.tables, c.k, c.v, c.D = [P + keep + 1] * B, dt.cpu(), kc.cpu(), vc.cpu(), D
+    c.k_norm = float(torch.nan_to_num(c.k.float()).norm(dim=-1).max())
+    ref, mag, weights = oracle(c, lyr.q.cpu(), [1] * B, D ** -0.5, lyr.w["sinks"].cpu(), lyr.window)
+    check(lyr.attn, ref, mag, F16, score_err(c, lyr.q.cpu(), D ** -0.5))
+    moved = scores - before
+    for b in range(B):
+        page, off = c.slots(b)
+        w = weights[b].t()[P:].float()
+        assert torch.allclose(moved.cpu()[page[P:], :, off[P:]], w, rtol=1e-3, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_gpu_capture_and_replay(m355, cuda):
+    """Both attentions and the eviction in one captured graph on a stream of its own, replayed with other contents, with eager
+    work between the replays, through one workspace; the results of an eager call every time."""
+    P, keep = 48, 40
+    c = Cache(77, [P + o for o in (300, 41, 7)], 8, 64, 16, F16, prefix=P, dst=P + keep)
+    kc, vc, bt, cl = c.device(cuda)
+    dst, q = c.dst.to(cuda), torch.empty((3, 64, 64), dtype=F16, device=cuda)
+    sc0 = c.scores.to(cuda)
+    need = max(m355.shared_prefix_attn_workspace_bytes(3, 3, 1, 64, 8, 64, 350, P), m355.paged_attn_decode_scored_workspace_bytes(3, 64, 8, 64, 350, P))
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    kept, lens = torch.empty((3, 8, keep), dtype=torch.int32, device=cuda), torch.empty(3, dtype=torch.int32, device=cuda)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    caches = [kc.clone(), vc.clone(), sc0.clone()]
+
+    def run():
+        m355.shared_prefix_attn(q, caches[0], caches[1], bt, cl, prefix_len=P, max_ctx=350, scale=0.125, workspace=ws, out=outs[0])
+        m355.paged_attn_decode_scored(q, caches[0], caches[1], caches[2], bt, cl, prefix_len=P, max_ctx=350, scale=0.125, workspace=ws, out=outs[1])
+        m355.kv_evict(*caches, bt, cl, dst, keep=keep, recent=3, prefix_len=P, max_ctx=350, kept=kept, new_lens=lens)
+
+    def load(seed, ctx):
+        q.copy_((1.5 * torch.randn(q.shape, generator=torch.Generator().manual_seed(seed))).to(F16))
+        cl.copy_(torch.tensor([P + o for o in ctx], dtype=torch.int32))
+        for t, s in zip(caches, (kc, vc, sc0)):
+            t.copy_(s)
+
+    load(0, (300, 41, 7))
+    c.tables = None
+    side = torch.cuda.Stream(device=cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        run()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            run()
+    torch.cuda.synchronize()
+    for seed, ctx in ((1, (300, 41, 7)), (2, (256, 40, 1)), (3, (0, 41, 7)), (4, (290, 13, 8))):
+        load(seed, ctx)
+        run()
+        torch.cuda.synchronize()
+        want = [t.clone() for t in outs + caches + [kept, lens]]
+        load(seed, ctx)
+        for t in outs + [kept, lens]:
+            t.zero_()
+        ws.fill_(255)                    # NaN patterns: nothing is read that the call has not written
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for got, exp in zip(outs + caches + [kept, lens], want):
+            assert torch.equal(got, exp)
+
+
+@pytest.mark.gpu
+def test_gpu_equals_the_paged_decode_kernel(m355, cuda):
+    """Without a prefix the new entry point computes what m355_paged_attn_decode_ex computes, and a batch whose rows name the
+    shared pages gives the same with and without prefix_len."""
+    P = 320
+    c = Cache(88, [P + o for o in (1, 200, 33, 90)], 8, 64, 16, F16, prefix=P)
+    q, sk = _inputs(c, 4, 64, 5, True)
+    kc, vc, bt, cl = c.device(cuda)
+    args = (q.to(cuda), kc, vc, bt, cl)
+    kw = dict(max_ctx=max(c.ctx), scale=0.125, sinks=sk.to(cuda))
+    want, mag, _ = oracle(c, q, [1] * 4, 0.125, sk)
+    for got in (m355.paged_attn_decode(*args, **kw), m355.shared_prefix_attn(*args, prefix_len=0, **kw),
+                m355.shared_prefix_attn(*args, prefix_len=P, **kw), m355.shared_prefix_attn(*args, prefix_len=P - 5, **kw)):
+        check(got, want, mag, F16, score_err(c, q, 0.125))
+
+
+@pytest.mark.gpu
+def test_gpu_bad_pages_stay_inside_the_cache(m355, cuda):
+    """Table entries far outside the cache are clamped: sequences with sound tables keep their results, nothing else in the
+    pool is written."""
+    c = Cache(99, [64, 50], 2, 64, 16, F16, dst=16)
+    q, _ = _inputs(c, 2, 8, 1, False)
+    kc, vc, bt, cl = c.device(cuda)
+    want, mag, _ = oracle(c, q, [1, 1], 0.125)
+    bad = bt.clone()
+    bad[1] = torch.tensor([1 << 30, -5, -(1 << 31), c.n], dtype=torch.int32)
+    sc = c.scores.to(cuda)
+    for got in (m355.shared_prefix_attn(q.to(cuda), kc, vc, bad, cl, prefix_len=0, max_ctx=64, scale=0.125),
+                m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bad, cl, max_ctx=64, scale=0.125)):
+        check(got[:1], want[:1], mag[:1], F16, score_err(c, q, 0.125))
+    page, off = c.slots(0)
+    rest = torch.ones((c.n, 16), dtype=torch.bool)
+    rest[page, off] = False
+    assert torch.equal(sc.cpu().transpose(1, 2)[rest], c.scores.transpose(1, 2)[rest])
+    dst = torch.full((2, 1), 1 << 20, dtype=torch.int32, device=cuda)
+    before = [t.clone() for t in (kc, vc, sc)]
+    _, lens = m355.kv_evict(kc, vc, sc, bad, cl, dst, keep=16, recent=2, max_ctx=64)
+    assert lens.tolist() == [16, 16] and all(torch.equal(a, b) for a, b in zip((kc, vc, sc), before))
+
+
+@pytest.mark.gpu
+def test_gpu_wrappers_refuse(m355, cuda):
+    c = Cache(1, [20, 30], 2, 64, 16, F16, dst=16)
+    kc, vc, bt, cl = c.device(cuda)
+    sc, q = c.scores.to(cuda), torch.zeros((2, 8, 64), dtype=F16, device=cuda)
+    call = lambda **kw: m355.shared_prefix_attn(*[kw.pop(n, d) for n, d in (("q", q), ("kc", kc), ("vc", vc), ("bt", bt), ("cl", cl))],      # noqa: E731
+                                                **dict(dict(prefix_len=0, max_ctx=32, scale=0.1), **kw))
+    for kw, err in ((dict(q=q.float()), TypeError), (dict(q=q.bfloat16()), TypeError), (dict(kc=kc.bfloat16()), TypeError),
+                    (dict(q=q[..., :32].contiguous()), ValueError), (dict(q=q.transpose(0, 1)), ValueError), (dict(kc=kc.transpose(0, 1)), ValueError),
+                    (dict(kc=kc[:, :, :, ::2], vc=vc[:, :, :, ::2]), ValueError), (dict(kc=torch.stack([kc, kc], 1)[:, 0]), ValueError),
+                    (dict(bt=bt.long()), TypeError), (dict(cl=cl[:1]), ValueError), (dict(sinks=torch.zeros(7, dtype=F16, device=cuda)), ValueError),
+                    (dict(sinks=torch.zeros(8, dtype=BF16, device=cuda)), TypeError), (dict(seq_starts=cl), ValueError),
+                    (dict(out=torch.zeros((2, 8, 32), dtype=F16, device=cuda)), ValueError), (dict(bt=bt.cpu()), m355.Mi355LibraryError),
+                    (dict(workspace=torch.zeros(16, dtype=torch.uint8, device=cuda)), m355.Mi355LibraryError), (dict(max_ctx=1000), m355.Mi355LibraryError)):
+        with pytest.raises(err):
+            call(**kw)
+    for bad in (sc[:, :1], sc.half(), sc.transpose(0, 1)):
+        with pytest.raises((ValueError, TypeError)):
+            m355.paged_attn_decode_scored(q, kc, vc, bad, bt, cl, max_ctx=32, scale=0.1)
+        with pytest.raises((ValueError, TypeError)):
+            m355.kv_evict(kc, vc, bad, bt, cl, c.dst.to(cuda), keep=16, recent=1, max_ctx=32)
+    with pytest.raises(ValueError):
+        m355.kv_evict(kc, vc, sc, bt, cl, c.dst[:1].to(cuda), keep=16, recent=1, max_ctx=32)
+    with pytest.raises(m355.Mi355LibraryError, match="new_lens"):
+        m355.kv_evict(kc, vc, sc, bt, cl, c.dst.to(cuda), keep=16, recent=1, max_ctx=32, new_lens=cl)
+    assert m355.shared_prefix_attn(q[:0], kc, vc, bt[:0], cl[:0], prefix_len=0, max_ctx=32, scale=0.1).shape == (0, 8, 64)
