@@ -778,41 +778,55 @@ def attn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: 
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}   # M355_DTYPE_F16, M355_DTYPE_BF16
 
 
-def _one_device(**tensors) -> None:
+def _one_device(names, *tensors) -> None:
     """All tensors on the GPU that is current: a launch goes to the current device's current stream."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2     # (a CPU tensor's get_device() is -1)
+    try:
+        if all(t is None or t.get_device() == current for t in tensors):
+            return
+    except AttributeError:
+        pass
+    for name, t in zip(names, tensors):
+        if t is not None and (not isinstance(t, torch.Tensor) or not t.is_cuda):
             raise Mi355LibraryError(f"{name} must be a GPU tensor; this path has no CPU implementation")
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != current:
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{current}")
+
+
+def _ptr(t: torch.Tensor, dtype: torch.dtype, name: str) -> int:
+    """_dev for a tensor that _one_device has seen."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
 def _token_rows(t: torch.Tensor, name: str, dtype: torch.dtype):
     """(pointer, token stride) of a [tokens][heads][D] tensor whose tokens may be strided."""
-    T, heads, D = t.shape
+    (T, heads, D), (st, sh, sd) = t.shape, t.stride()
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if (D > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != D):
+    if (D > 1 and sd != 1) or (heads > 1 and sh != D):
         raise ValueError(f"{name} must have contiguous heads")
-    return t.data_ptr(), t.stride(0) if T > 1 else heads * D
+    return t.data_ptr(), st if T > 1 else heads * D
 
 
 def _paged_cache(kcache: torch.Tensor, vcache: torch.Tensor, dtype: torch.dtype) -> int:
     """Page stride in elements of caches [blocks][block_size][Hkv][D]; pages may be strided (K and V of one page side by
     side, say), a page itself is contiguous."""
-    if kcache.dim() != 4 or kcache.shape != vcache.shape:
+    shape, ks, vs = kcache.shape, kcache.stride(), vcache.stride()
+    if len(shape) != 4 or shape != vcache.shape:
         raise ValueError("caches must be [blocks][block_size][Hkv][D], both alike")
     if kcache.dtype != dtype or vcache.dtype != dtype:
         raise TypeError(f"caches must be {dtype}, got {kcache.dtype} and {vcache.dtype}")
-    n, bs, hkv, d = kcache.shape
-    for name, t in (("kcache", kcache), ("vcache", vcache)):
-        if (d > 1 and t.stride(3) != 1) or (hkv > 1 and t.stride(2) != d) or (bs > 1 and t.stride(1) != hkv * d):
+    n, bs, hkv, d = shape
+    for name, (_, s1, s2, s3) in (("kcache", ks), ("vcache", vs)):
+        if (d > 1 and s3 != 1) or (hkv > 1 and s2 != d) or (bs > 1 and s1 != hkv * d):
             raise ValueError(f"{name}: a page must be contiguous")
-    if n > 1 and kcache.stride(0) != vcache.stride(0):
+    if n > 1 and ks[0] != vs[0]:
         raise ValueError("caches must share their page stride")
-    return kcache.stride(0) if n > 1 else bs * hkv * d
+    return ks[0] if n > 1 else bs * hkv * d
 
 
 def shared_prefix_attn_workspace_bytes(T: int, B: int, max_q: int, Hq: int, Hkv: int, D: int, max_ctx: int, prefix_len: int) -> int:
@@ -827,8 +841,8 @@ def shared_prefix_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
     tokens, read through row 0 of block_tables, all sequences share.  seq_starts int32 [B + 1] gives the sequences' tokens,
     max_q the longest one's number; without it there is one token per sequence.  ctx_lens count the new tokens.
     m355_shared_prefix_attn."""
-    _one_device(q=q, kcache=kcache, vcache=vcache, block_tables=block_tables, ctx_lens=ctx_lens, seq_starts=seq_starts, sinks=sinks,
-                workspace=workspace, out=out)
+    _one_device(("q", "kcache", "vcache", "block_tables", "ctx_lens", "seq_starts", "sinks", "workspace", "out"), q, kcache, vcache,
+                block_tables, ctx_lens, seq_starts, sinks, workspace, out)
     if q.dtype not in _DTYPE_CODES:
         raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
     T, Hq, D = q.shape
@@ -852,10 +866,10 @@ def shared_prefix_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         workspace = torch.empty(max(256, shared_prefix_attn_workspace_bytes(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len)), dtype=torch.uint8,
                                 device=q.device)
     _check(load().m355_shared_prefix_attn(
-        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _dev(block_tables, torch.int32, "block_tables"), _dev(ctx_lens, torch.int32, "ctx_lens"),
-        None if seq_starts is None else _dev(seq_starts, torch.int32, "seq_starts"), T, B, int(max_q), Hq, Hkv, D, _DTYPE_CODES[q.dtype],
+        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _ptr(block_tables, torch.int32, "block_tables"), _ptr(ctx_lens, torch.int32, "ctx_lens"),
+        None if seq_starts is None else _ptr(seq_starts, torch.int32, "seq_starts"), T, B, int(max_q), Hq, Hkv, D, _DTYPE_CODES[q.dtype],
         nblocks, block_size, max_blocks, stride, int(max_ctx), int(prefix_len), q_stride, o_stride, float(scale),
-        None if sinks is None else _dev(sinks, q.dtype, "sinks"), int(window), _dev(workspace, torch.uint8, "workspace"), workspace.numel(),
+        None if sinks is None else _ptr(sinks, q.dtype, "sinks"), int(window), _ptr(workspace, torch.uint8, "workspace"), workspace.numel(),
         o_ptr, _stream()), "m355_shared_prefix_attn")
     return out
 
@@ -868,7 +882,7 @@ def _page_scores(scores: torch.Tensor, kcache: torch.Tensor) -> int:
     nblocks, block_size, Hkv, _ = kcache.shape
     if tuple(scores.shape) != (nblocks, Hkv, block_size):
         raise ValueError(f"scores is {tuple(scores.shape)}, expected {(nblocks, Hkv, block_size)}")
-    return _dev(scores, torch.float32, "scores")
+    return _ptr(scores, torch.float32, "scores")
 
 
 def paged_attn_decode_scored(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, scores: torch.Tensor, block_tables: torch.Tensor,
@@ -878,8 +892,8 @@ def paged_attn_decode_scored(q: torch.Tensor, kcache: torch.Tensor, vcache: torc
     """shared_prefix_attn with one token per sequence, which also adds the attention weight of every own token (positions
     from prefix_len on), summed over a KV head's query heads, to scores [blocks][Hkv][block_size] fp32.  Zero a page's
     scores when the page is handed out.  m355_paged_attn_decode_scored."""
-    _one_device(q=q, kcache=kcache, vcache=vcache, scores=scores, block_tables=block_tables, ctx_lens=ctx_lens, sinks=sinks,
-                workspace=workspace, out=out)
+    _one_device(("q", "kcache", "vcache", "scores", "block_tables", "ctx_lens", "sinks", "workspace", "out"), q, kcache, vcache, scores,
+                block_tables, ctx_lens, sinks, workspace, out)
     if q.dtype not in _DTYPE_CODES:
         raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
     B, Hq, D = q.shape
@@ -901,10 +915,10 @@ def paged_attn_decode_scored(q: torch.Tensor, kcache: torch.Tensor, vcache: torc
         workspace = torch.empty(max(256, paged_attn_decode_scored_workspace_bytes(B, Hq, Hkv, D, max_ctx, prefix_len)), dtype=torch.uint8,
                                 device=q.device)
     _check(load().m355_paged_attn_decode_scored(
-        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _dev(block_tables, torch.int32, "block_tables"),
-        _dev(ctx_lens, torch.int32, "ctx_lens"), B, Hq, Hkv, D, _DTYPE_CODES[q.dtype], nblocks, block_size, block_tables.shape[1], stride,
-        int(max_ctx), int(prefix_len), q_stride, o_stride, float(scale), None if sinks is None else _dev(sinks, q.dtype, "sinks"),
-        int(window), _dev(workspace, torch.uint8, "workspace"), workspace.numel(), o_ptr, _stream()), "m355_paged_attn_decode_scored")
+        q_ptr, kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _ptr(block_tables, torch.int32, "block_tables"),
+        _ptr(ctx_lens, torch.int32, "ctx_lens"), B, Hq, Hkv, D, _DTYPE_CODES[q.dtype], nblocks, block_size, block_tables.shape[1], stride,
+        int(max_ctx), int(prefix_len), q_stride, o_stride, float(scale), None if sinks is None else _ptr(sinks, q.dtype, "sinks"),
+        int(window), _ptr(workspace, torch.uint8, "workspace"), workspace.numel(), o_ptr, _stream()), "m355_paged_attn_decode_scored")
     return out
 
 
@@ -914,8 +928,8 @@ def kv_evict(kcache: torch.Tensor, vcache: torch.Tensor, scores: torch.Tensor, b
     """Per sequence and KV head: of the tokens behind prefix_len the last `recent` and the best-scored others, `keep` in all,
     copied in order with their scores to the pages of dst_tables (other pages of the same cache).  Returns (kept positions
     [B][Hkv][keep], -1 behind the last; new context lengths [B]).  m355_kv_evict."""
-    _one_device(kcache=kcache, vcache=vcache, scores=scores, block_tables=block_tables, ctx_lens=ctx_lens, dst_tables=dst_tables, kept=kept,
-                new_lens=new_lens)
+    _one_device(("kcache", "vcache", "scores", "block_tables", "ctx_lens", "dst_tables", "kept", "new_lens"), kcache, vcache, scores,
+                block_tables, ctx_lens, dst_tables, kept, new_lens)
     B, max_blocks = block_tables.shape
     nblocks, block_size, Hkv, D = kcache.shape
     if ctx_lens.numel() != B or dst_tables.shape[0] != B:
@@ -930,8 +944,8 @@ def kv_evict(kcache: torch.Tensor, vcache: torch.Tensor, scores: torch.Tensor, b
     elif new_lens.numel() != B:
         raise ValueError(f"new_lens has {new_lens.numel()} entries, expected {B}")
     _check(load().m355_kv_evict(
-        kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _dev(block_tables, torch.int32, "block_tables"),
-        _dev(ctx_lens, torch.int32, "ctx_lens"), _dev(dst_tables, torch.int32, "dst_tables"), B, Hkv, D * size, nblocks, block_size,
-        max_blocks, dst_tables.shape[1], stride * size, int(max_ctx), int(prefix_len), int(keep), int(recent), _dev(kept, torch.int32, "kept"),
-        _dev(new_lens, torch.int32, "new_lens"), _stream()), "m355_kv_evict")
+        kcache.data_ptr(), vcache.data_ptr(), _page_scores(scores, kcache), _ptr(block_tables, torch.int32, "block_tables"),
+        _ptr(ctx_lens, torch.int32, "ctx_lens"), _ptr(dst_tables, torch.int32, "dst_tables"), B, Hkv, D * size, nblocks, block_size,
+        max_blocks, dst_tables.shape[1], stride * size, int(max_ctx), int(prefix_len), int(keep), int(recent), _ptr(kept, torch.int32, "kept"),
+        _ptr(new_lens, torch.int32, "new_lens"), _stream()), "m355_kv_evict")
     return kept, new_lens
