@@ -33,133 +33,375 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Each wave looks after a run of consecutive tokens, 64 of them at a time, so that kept positions come out in order from
-// ballots alone.  ITEMS: keys per lane that stay in registers (0: they are read again for every pass).
-constexpr int EV_BINS = 2048;
-template <int THREADS, int ITEMS>
-__global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
-    constexpr int WAVES = THREADS / 64;
-    __shared__ int hist[EV_BINS];
-    __shared__ int wave_sum_of[WAVES], wave_gt[WAVES], wave_eq[WAVES];
-    __shared__ uint32_t sh_prefix;
-    __shared__ int sh_left;
-    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// What a selection works on, and the part of it that needs no selection: lengths, the last tokens, the filler.
+struct Selection {
+    int cand, c;   // c of the first cand own tokens are to be found
+    int32_t* kept;
+    const int32_t* table;
+};
+template <int THREADS>
+__device__ __forceinline__ bool begin_selection(const EvictArgs& a, int hk, int b, Selection& s) {
+    const int tid = threadIdx.x;
     const int ctx = min(max(a.ctx_lens[b], 0), a.max_ctx), n = ctx - a.prefix_len;
-    int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hk) * a.keep;
     const int m = min(max(n, 0), a.keep);
+    s.kept = a.kept + ((int64_t)b * a.Hkv + hk) * a.keep;
+    s.table = a.tables + (int64_t)b * a.max_blocks;
     if (hk == 0 && tid == 0) a.new_lens[b] = n > 0 ? a.prefix_len + m : ctx;
-    for (int i = m + tid; i < a.keep; i += THREADS) kept[i] = -1;
+    for (int i = m + tid; i < a.keep; i += THREADS) s.kept[i] = -1;
     if (n <= a.keep) {
-        for (int i = tid; i < m; i += THREADS) kept[i] = a.prefix_len + i;
-        return;
+        for (int i = tid; i < m; i += THREADS) s.kept[i] = a.prefix_len + i;
+        return false;
     }
-    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    const int cand = n - a.recent, c = a.keep - a.recent;   // cand > c: there is something to leave out
-    for (int i = tid; i < a.recent; i += THREADS) kept[c + i] = a.prefix_len + cand + i;
-    if (c == 0) return;
-    const int steps = (cand + THREADS - 1) / THREADS, first = wave * steps * 64 + lane;   // lane's token of step j: first + 64 j
-    auto score_at = [&](int i, int page, int blk) {
-        const int pos = a.prefix_len + min(i, cand - 1);
-        return a.scores[((int64_t)min(max(blk, 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + (pos - page * a.block_size)];
-    };
-    uint32_t key[ITEMS ? ITEMS : 1];
-    if constexpr (ITEMS > 0) {
-        constexpr int G = ITEMS < 16 ? ITEMS : 16;   // page numbers, then scores on their way at a time
+    s.cand = n - a.recent, s.c = a.keep - a.recent;   // cand > c: there is something to leave out
+    for (int i = tid; i < a.recent; i += THREADS) s.kept[s.c + i] = a.prefix_len + s.cand + i;
+    return s.c > 0;
+}
+__device__ __forceinline__ uint32_t key_at(const EvictArgs& a, const Selection& s, int hk, int i) {
+    const int pos = a.prefix_len + min(i, s.cand - 1), page = page_of(a, pos), blk = min(max(s.table[page], 0), a.num_blocks - 1);
+    return score_key(a.scores[((int64_t)blk * a.Hkv + hk) * a.block_size + (pos - page * a.block_size)]);
+}
+
+// f(step, key) for the wave's steps [0, steps) (token first + 64 step), EV_GROUP page numbers and then scores on their way
+// at a time.  Steps behind the last one come with step = -1.
+constexpr int EV_GROUP = 8;
+template <typename F>
+__device__ __forceinline__ void each_key(const EvictArgs& a, const Selection& s, int hk, int first, int steps, F f) {
+    for (int j0 = 0; j0 < steps; j0 += EV_GROUP) {
+        int off[EV_GROUP], blk[EV_GROUP];
+        float score[EV_GROUP];
 #pragma unroll
-        for (int j0 = 0; j0 < ITEMS; j0 += G) {
-            if (j0 >= steps) break;
-            int page[G], blk[G];
+        for (int j = 0; j < EV_GROUP; j++) {
+            const int pos = a.prefix_len + min(first + 64 * (j0 + j), s.cand - 1), page = page_of(a, pos);
+            off[j] = pos - page * a.block_size;
+            blk[j] = s.table[page];
+        }
 #pragma unroll
-            for (int j = 0; j < G; j++) {
-                page[j] = page_of(a, a.prefix_len + min(first + 64 * (j0 + j), cand - 1));
-                blk[j] = table[page[j]];
+        for (int j = 0; j < EV_GROUP; j++)
+            score[j] = a.scores[((int64_t)min(max(blk[j], 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + off[j]];
+#pragma unroll
+        for (int j = 0; j < EV_GROUP; j++) f(j0 + j < steps ? j0 + j : -1, score_key(score[j]));
+    }
+}
+
+__device__ __forceinline__ bool aligned_scores(const EvictArgs& a) { return (reinterpret_cast<uintptr_t>(a.scores) & 15) == 0; }
+
+// The bin of the left-th largest of the values counted in hist[0 .. bins); left becomes its rank within that bin.  Called by
+// all threads behind a barrier; ends with one.
+template <int THREADS, int BINS>
+__device__ __forceinline__ int find_bin(const int* hist, int& left) {
+    constexpr int PER = (BINS + THREADS - 1) / THREADS;   // bins per thread, the topmost ones first
+    __shared__ int wave_sum_of[THREADS / 64], found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (tid * PER + i < BINS) mine += hist[BINS - 1 - (tid * PER + i)];
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int v = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 63) wave_sum_of[wave] = incl;
+    __syncthreads();
+    int above = incl - mine;   // values in the bins above this thread's
+    for (int w = 0; w < wave; w++) above += wave_sum_of[w];
+    if (above < left && above + mine >= left) {   // exactly one thread
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int bin = BINS - 1 - (tid * PER + i), h = hist[bin];
+            if (above + h >= left) {
+                found[0] = bin;
+                found[1] = left - above;
+                break;
             }
-#pragma unroll
-            for (int j = 0; j < G; j++) key[j0 + j] = score_key(score_at(first + 64 * (j0 + j), page[j], blk[j]));
+            above += h;
         }
     }
-    auto each = [&](auto f) {   // f(token, key, is it a candidate) for every step of the wave
-        if constexpr (ITEMS > 0) {
-#pragma unroll
-            for (int j = 0; j < ITEMS; j++)
-                if (j < steps) f(first + 64 * j, key[j], first + 64 * j < cand);
-        } else {
-            for (int j = 0; j < steps; j++) {
-                const int i = first + 64 * j;
-                const int page = page_of(a, a.prefix_len + min(i, cand - 1));
-                f(i, score_key(score_at(i, page, table[page])), i < cand);
-            }
-        }
-    };
-    uint32_t prefix = 0;   // the leading bits of the c-th largest key, found so far
-    int left = c;          // how many of the keys with those leading bits are wanted
-#pragma unroll
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
-        for (int i = tid; i < EV_BINS; i += THREADS) hist[i] = 0;
-        __syncthreads();
-        each([&](int, uint32_t k, bool in) {
-            if (in && (pass == 0 || (k >> (shift + width)) == (prefix >> (shift + width)))) atomicAdd(&hist[(k >> shift) & ((1 << width) - 1)], 1);
-        });
-        __syncthreads();
-        // the bin of the left-th largest: thread t looks after PER bins, the topmost ones first
-        constexpr int PER = EV_BINS / THREADS;
-        int mine = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++) mine += hist[EV_BINS - 1 - (tid * PER + i)];
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int v = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += v;
-        }
-        if (lane == 63) wave_sum_of[wave] = incl;
-        __syncthreads();
-        int above = incl - mine;   // keys in the bins above this thread's
-        for (int w = 0; w < wave; w++) above += wave_sum_of[w];
-        if (above < left && above + mine >= left) {   // exactly one thread
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const int bin = EV_BINS - 1 - (tid * PER + i), h = hist[bin];
-                if (above < left && above + h >= left) {
-                    sh_prefix = prefix | ((uint32_t)bin << shift);
-                    sh_left = left - above;
-                    break;
-                }
-                above += h;
-            }
-        }
-        __syncthreads();
-        prefix = sh_prefix;
-        left = sh_left;
-    }
-    // prefix is the c-th largest key: all above it and the first `left` equal to it
+    __syncthreads();
+    left = found[1];
+    const int bin = found[0];
+    __syncthreads();
+    return bin;
+}
+template <int THREADS>
+__device__ __forceinline__ void clear_bins(int* hist, int bins) {
+    for (int i = threadIdx.x; i < bins; i += THREADS) hist[i] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ int lanes_below(uint64_t votes) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(votes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)votes, 0));
+}
+
+// Lists in order the candidates above `limit` and the first `left` equal to it.  Each wave looks after a run of consecutive
+// tokens, 64 of them at a time, so that positions come out in order from ballots alone; each(f) calls f(token, above, equal)
+// for the wave's steps.
+template <int THREADS, typename EACH>
+__device__ __forceinline__ void list_kept(const EvictArgs& a, int32_t* kept, int left, EACH each) {
+    __shared__ int wave_gt[THREADS / 64], wave_eq[THREADS / 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int gt = 0, eq = 0;
-    each([&](int, uint32_t k, bool in) {
-        gt += __popcll(__ballot(in && k > prefix));
-        eq += __popcll(__ballot(in && k == prefix));
+    each([&](int, bool above, bool equal) {
+        gt += __popcll(__ballot(above));
+        eq += __popcll(__ballot(equal));
     });
     if (lane == 0) {
         wave_gt[wave] = gt;
         wave_eq[wave] = eq;
     }
     __syncthreads();
-    int at = 0, equal = 0;   // kept before this wave; equal ones seen before it
+    int at = 0, seen = 0;   // kept before this wave; equal ones seen before it
     for (int w = 0; w < wave; w++) {
         at += wave_gt[w];
-        equal += wave_eq[w];
+        seen += wave_eq[w];
     }
-    at += min(equal, left);
-    auto below = [](uint64_t votes) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(votes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)votes, 0)); };
-    each([&](int i, uint32_t k, bool in) {
-        bool take = in && k > prefix;
-        const uint64_t eqs = __ballot(in && k == prefix);
-        if (eqs && equal < left) take |= in && k == prefix && equal + below(eqs) < left;
-        equal += __popcll(eqs);
+    at += min(seen, left);
+    each([&](int i, bool above, bool equal) {
+        const uint64_t eqs = __ballot(equal);
+        const bool take = above || (equal && seen + lanes_below(eqs) < left);
+        seen += __popcll(eqs);
         const uint64_t takes = __ballot(take);
-        if (take) kept[at + below(takes)] = a.prefix_len + i;
+        if (take) kept[at + lanes_below(takes)] = a.prefix_len + i;
         at += __popcll(takes);
+    });
+}
+
+// Up to THREADS * ITEMS own tokens, their keys in registers (ITEMS = 0: any number, keys are read again for every pass).
+template <int THREADS, int ITEMS>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
+    __shared__ int hist[2048];
+    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Selection s;
+    if (!begin_selection<THREADS>(a, hk, b, s)) return;
+    const int steps = (s.cand + THREADS - 1) / THREADS, first = wave * steps * 64 + lane;   // lane's token of step j: first + 64 j
+    uint32_t key[ITEMS ? ITEMS : 1];
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++)
+        if (j < steps) key[j] = key_at(a, s, hk, first + 64 * j);
+    auto each = [&](auto f) {   // f(token, key, is it a candidate) for every step of the wave
+        if constexpr (ITEMS > 0) {
+#pragma unroll
+            for (int j = 0; j < ITEMS; j++)
+                if (j < steps) f(first + 64 * j, key[j], first + 64 * j < s.cand);
+        } else {
+            each_key(a, s, hk, first, steps, [&](int j, uint32_t k) { f(first + 64 * j, k, j >= 0 && first + 64 * j < s.cand); });
+        }
+    };
+    int left = s.c;
+    clear_bins<THREADS>(hist, 2048);
+    each([&](int, uint32_t k, bool in) {
+        if (in) atomicAdd(&hist[k >> 21], 1);
+    });
+    __syncthreads();
+    uint32_t limit = find_bin<THREADS, 2048>(hist, left);
+    clear_bins<THREADS>(hist, 2048);
+    each([&](int, uint32_t k, bool in) {
+        if (in && k >> 21 == limit) atomicAdd(&hist[k >> 10 & 2047], 1);
+    });
+    __syncthreads();
+    limit = limit << 11 | find_bin<THREADS, 2048>(hist, left);
+    clear_bins<THREADS>(hist, 1024);
+    each([&](int, uint32_t k, bool in) {
+        if (in && k >> 10 == limit) atomicAdd(&hist[k & 1023], 1);
+    });
+    __syncthreads();
+    limit = limit << 10 | find_bin<THREADS, 1024>(hist, left);
+    list_kept<THREADS>(a, s.kept, left, [&](auto f) { each([&](int i, uint32_t k, bool in) { f(i, in && k > limit, in && k == limit); }); });
+}
+
+// Exclusive prefix sum over the wave, and its total.
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v, int& total) {
+    int s = dpp_add<0x111>(v);     // row_shr:1, 2, 4, 8: inclusive sums within 16 lanes
+    s = dpp_add<0x112>(s);
+    s = dpp_add<0x114>(s);
+    s = dpp_add<0x118>(s);
+    s = dpp_add<0x142, 0xa>(s);    // row_bcast15 into rows 1 and 3
+    s = dpp_add<0x143, 0xc>(s);    // row_bcast31 into rows 2 and 3
+    total = __builtin_amdgcn_readlane(s, 63);
+    return s - v;
+}
+
+// Up to N own tokens: the upper halves of their keys stay in LDS, eight tokens to a lane's 16 bytes, 512 to a wave's block.
+// Once the limit's upper half is known, only the few keys that share it are needed whole: each wave lists its own ones in
+// order and reads them once more, all together, so that their lower halves are at hand wherever the wave comes across them
+// again.  Where equal scores make them too many for the lists, they are read again each time.
+constexpr int EV_LONG = 65536, EV_LIST = 256;
+template <int N>
+__global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
+    constexpr int THREADS = 1024, WAVES = THREADS / 64;
+    __shared__ __attribute__((aligned(16))) uint16_t upper[N];
+    __shared__ uint16_t list_at[WAVES][EV_LIST], list_low[WAVES][EV_LIST];
+    __shared__ int hist[2048], too_many, wave_gt[WAVES], wave_eq[WAVES];
+    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Selection s;
+    if (!begin_selection<THREADS>(a, hk, b, s)) return;
+    const int blocks = (s.cand + WAVES * 512 - 1) / (WAVES * 512), run = wave * blocks * 512;   // this wave's first token
+    if (tid == 0) too_many = 0;
+    clear_bins<THREADS>(hist, 2048);
+    {
+        // pages of a multiple of 8 tokens: a lane's eight scores lie side by side (own tokens start on a page)
+        const bool vec = a.block_size % 8 == 0 && aligned_scores(a);
+        for (int q0 = 0; q0 < blocks; q0 += 4) {
+            float sc[4][8];
+            if (vec) {
+                int off[4], blk[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int i = min(run + (q0 + q) * 512 + lane * 8, (s.cand - 1) & ~7), pos = a.prefix_len + i, page = page_of(a, pos);
+                    off[q] = pos - page * a.block_size;
+                    blk[q] = s.table[page];
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float4_t* from = reinterpret_cast<const float4_t*>(
+                        a.scores + ((int64_t)min(max(blk[q], 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + off[q]);
+                    const float4_t x = from[0], y = from[1];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[q][e] = x[e], sc[q][4 + e] = y[e];
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int pos = a.prefix_len + min(run + (q0 + q) * 512 + lane * 8 + e, s.cand - 1), page = page_of(a, pos);
+                        const int blk = min(max(s.table[page], 0), a.num_blocks - 1);
+                        sc[q][e] = a.scores[((int64_t)blk * a.Hkv + hk) * a.block_size + (pos - page * a.block_size)];
+                    }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (q0 + q >= blocks) break;
+                const int i = run + (q0 + q) * 512 + lane * 8;
+                u32x4_t packed;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const uint32_t k0 = score_key(sc[q][e]), k1 = score_key(sc[q][e + 1]);
+                    packed[e / 2] = k0 >> 16 | (k1 & 0xffff0000u);
+                    if (i + e < s.cand) atomicAdd(&hist[k0 >> 21], 1);
+                    if (i + e + 1 < s.cand) atomicAdd(&hist[k1 >> 21], 1);
+                }
+                if (i < s.cand) *reinterpret_cast<u32x4_t*>(upper + i) = packed;   // (N is a multiple of 8)
+            }
+        }
+    }
+    __syncthreads();
+    auto each = [&](auto f) {   // f(first token, eight upper halves, how many of them are candidates) for the wave's blocks
+        for (int q = 0; q < blocks; q++) {
+            const int i = run + q * 512 + lane * 8;
+            const u32x4_t u = *reinterpret_cast<const u32x4_t*>(upper + min(i, (s.cand - 1) & ~7));
+            f(i, u, min(max(s.cand - i, 0), 8));
+        }
+    };
+    auto half = [](u32x4_t u, int e) { return e & 1 ? u[e / 2] >> 16 : u[e / 2] & 0xffffu; };
+    auto equal_to = [&](u32x4_t u, uint32_t t, int n) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) m |= half(u, e) == t ? 1u << e : 0u;
+        return m & ((1u << n) - 1);
+    };
+    int left = s.c;
+    uint32_t top = find_bin<THREADS, 2048>(hist, left);
+    clear_bins<THREADS>(hist, 32);
+    each([&](int, u32x4_t u, int n) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n && half(u, e) >> 5 == top) atomicAdd(&hist[half(u, e) & 31], 1);
+    });
+    __syncthreads();
+    top = top << 5 | find_bin<THREADS, 32>(hist, left);
+    int mine = 0;   // of this wave's keys, how many have the limit's upper half
+    each([&](int i, u32x4_t u, int n) {
+        const uint32_t eq = equal_to(u, top, n);
+        if (!__any(eq != 0)) return;
+        int total, at = mine + wave_scan(__popc(eq), total);
+        for (uint32_t m = eq; m; m &= m - 1, at++)
+            if (at < EV_LIST) list_at[wave][at] = (uint16_t)(i - run + __builtin_ctz(m));
+        mine += total;
+    });
+    if (mine > EV_LIST) too_many = 1;
+    __syncthreads();
+    const bool listed = !too_many;
+    if (listed)
+        for (int e = lane; e < mine; e += 64) list_low[wave][e] = (uint16_t)key_at(a, s, hk, run + list_at[wave][e]);
+    __syncthreads();
+    auto each_low = [&](auto f) {   // f(lower half) of every key whose upper half is the limit's
+        if (listed) {
+            for (int e = lane; e < mine; e += 64) f((uint32_t)list_low[wave][e]);
+        } else {
+            each([&](int i, u32x4_t u, int n) {
+                for (uint32_t m = equal_to(u, top, n); m; m &= m - 1) f(key_at(a, s, hk, i + __builtin_ctz(m)) & 0xffffu);
+            });
+        }
+    };
+    clear_bins<THREADS>(hist, 256);
+    each_low([&](uint32_t l) { atomicAdd(&hist[l >> 8], 1); });
+    __syncthreads();
+    uint32_t low = find_bin<THREADS, 256>(hist, left);
+    clear_bins<THREADS>(hist, 256);
+    each_low([&](uint32_t l) {
+        if (l >> 8 == low) atomicAdd(&hist[l & 255], 1);
+    });
+    __syncthreads();
+    low = low << 8 | find_bin<THREADS, 256>(hist, left);
+
+    // f(first token, mask of the eight that lie above the limit, mask of those equal to it)
+    auto judged = [&](auto f) {
+        int met = 0;
+        each([&](int i, u32x4_t u, int n) {
+            uint32_t above = 0, equal = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) above |= half(u, e) > top ? 1u << e : 0u;
+            above &= (1u << n) - 1;
+            const uint32_t eq = equal_to(u, top, n);
+            if (__any(eq != 0)) {
+                int total, at = met + wave_scan(__popc(eq), total);
+                for (uint32_t m = eq; m; m &= m - 1, at++) {
+                    const int e = __builtin_ctz(m);
+                    const uint32_t l = listed ? (uint32_t)list_low[wave][at] : key_at(a, s, hk, i + e) & 0xffffu;
+                    above |= l > low ? 1u << e : 0u;
+                    equal |= l == low ? 1u << e : 0u;
+                }
+                met += total;
+            }
+            f(i, above, equal);
+        });
+    };
+    int gt = 0, eq = 0;
+    judged([&](int, uint32_t above, uint32_t equal) {
+        gt += __popc(above);
+        eq += __popc(equal);
+    });
+    int gt_all, eq_all;
+    wave_scan(gt, gt_all), wave_scan(eq, eq_all);
+    if (lane == 0) {
+        wave_gt[wave] = gt_all;
+        wave_eq[wave] = eq_all;
+    }
+    __syncthreads();
+    int at = 0, seen = 0;   // kept before this wave; equal ones seen before it
+    for (int w = 0; w < wave; w++) {
+        at += wave_gt[w];
+        seen += wave_eq[w];
+    }
+    at += min(seen, left);
+    judged([&](int i, uint32_t above, uint32_t equal) {
+        if (__any(equal != 0)) {   // the first `left` equal ones
+            int total, rank = seen + wave_scan(__popc(equal), total);
+            for (uint32_t m = equal; m; m &= m - 1, rank++)
+                if (rank < left) above |= m & -m;
+            seen += total;
+        }
+        int total;
+        int32_t* to = s.kept + at + wave_scan(__popc(above), total);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (above >> e & 1) *to++ = a.prefix_len + i + e;
+        at += total;
     });
 }
 
@@ -231,8 +473,8 @@ extern "C" int m355_kv_evict(void* kcache, void* vcache, float* scores, const in
     hipStream_t st = (hipStream_t)stream;
     const int64_t own = max_ctx - (int64_t)prefix_len;
     if (own <= 1024) kv_select_kernel<256, 4><<<B * Hkv, 256, 0, st>>>(a);
-    else if (own <= 16384) kv_select_kernel<1024, 16><<<B * Hkv, 1024, 0, st>>>(a);
-    else if (own <= 65536) kv_select_kernel<1024, 64><<<B * Hkv, 1024, 0, st>>>(a);
+    else if (own <= 16384) kv_select_long_kernel<16384><<<B * Hkv, 1024, 0, st>>>(a);
+    else if (own <= EV_LONG) kv_select_long_kernel<EV_LONG><<<B * Hkv, 1024, 0, st>>>(a);
     else kv_select_kernel<1024, 0><<<B * Hkv, 1024, 0, st>>>(a);
     M355_LAUNCH_CHECK("kv_select_kernel");
     if (chunks) {

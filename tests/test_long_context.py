@@ -245,7 +245,8 @@ def test_gpu_scored_decode(layout, case, m355, cuda):
 
 EVICT = [([1], 0, 16, 4, 1), ([5, 6, 7], 0, 16, 6, 2), ([100, 300, 129], 32, 16, 64, 10), ([1000, 17], 0, 20, 33, 33),
          ([700, 300], 64, 64, 256, 0), ([4, 2], 16, 16, 1, 0), ([3000, 64], 0, 128, 1025, 100), ([0, 9], 48, 16, 8, 3),
-         ([1024, 1025], 0, 16, 500, 1), ([17000, 16384], 64, 64, 3333, 128), ([66000, 1], 0, 128, 4097, 5)]
+         ([1024, 1025], 0, 16, 500, 1), ([17000, 16384], 64, 64, 3333, 128), ([66000, 1], 0, 128, 4097, 5),
+         ([3000, 2001], 40, 20, 700, 7), ([40001, 19000], 0, 64, 10000, 77)]
 
 
 def evict_oracle(c, keep, recent):
@@ -299,7 +300,9 @@ def test_gpu_kv_evict(case, kind, m355, cuda):
             page, off = c.slots(b, kept[b, h, :m].long())
             exp[0][tp, tf, h], exp[1][tp, tf, h], exp[2][tp, h, tf] = c.k[page, off, h], c.v[page, off, h], c.scores[page, h, off]
     kc, vc, bt, cl = c.device(cuda)
-    sc, dst = c.scores.to(cuda), c.dst.to(cuda)
+    dst = c.dst.to(cuda)
+    sc = torch.empty(c.scores.numel() + 1, device=cuda)[case % 2:][:c.scores.numel()].view(c.scores.shape)    # (4-byte aligned, too)
+    sc.copy_(c.scores)
     for _ in range(2):                          # the source pages stay: a second call does the same again
         got_kept, got_lens = m355.kv_evict(kc, vc, sc, bt, cl, dst, keep=keep, recent=recent, prefix_len=P, max_ctx=max(c.ctx))
         assert torch.equal(got_kept.cpu(), kept)
