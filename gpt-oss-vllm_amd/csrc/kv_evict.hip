@@ -405,28 +405,46 @@ __global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
     });
 }
 
-// A workgroup per (sequence, KV head, EV_ROWS kept tokens).
-constexpr int EV_ROWS = 64;
+// A workgroup per (sequence, KV head, EV_ROWS kept tokens); a lane has EV_AHEAD 16-byte pieces of K and of V on their way.
+constexpr int EV_ROWS = 32, EV_AHEAD = 2;
 __global__ __launch_bounds__(EV_THREADS) void kv_move_kernel(EvictArgs a, int chunks) {
     const int hk = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv % chunks, b = blockIdx.x / a.Hkv / chunks, tid = threadIdx.x;
     const int m = a.new_lens[b] - a.prefix_len;
     const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hk) * a.keep;
     const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
     const int32_t* dst = a.dst_tables + (int64_t)b * a.max_dst_blocks;
-    const int pieces = a.row_bytes / 16, i0 = chunk * EV_ROWS, rows = min(EV_ROWS, m - i0);
-    for (int w = tid; w < rows * pieces; w += EV_THREADS) {
-        const int i = i0 + w / pieces, off = (w % pieces) * 16;
-        const int from = kept[i], to = a.prefix_len + i;
-        const int fp = page_of(a, from), tp = page_of(a, to);
-        const int fb = min(max(table[fp], 0), a.num_blocks - 1), tb = dst[tp];
-        if (tb < 0 || tb >= a.num_blocks) continue;
-        const int64_t src = fb * a.block_stride + ((int64_t)(from - fp * a.block_size) * a.Hkv + hk) * a.row_bytes + off;
-        const int64_t put = tb * a.block_stride + ((int64_t)(to - tp * a.block_size) * a.Hkv + hk) * a.row_bytes + off;
-        *reinterpret_cast<u32x4_t*>(a.kc + put) = *reinterpret_cast<const u32x4_t*>(a.kc + src);
-        *reinterpret_cast<u32x4_t*>(a.vc + put) = *reinterpret_cast<const u32x4_t*>(a.vc + src);
-        if (off == 0)
-            a.scores[((int64_t)tb * a.Hkv + hk) * a.block_size + (to - tp * a.block_size)] =
-                a.scores[((int64_t)fb * a.Hkv + hk) * a.block_size + (from - fp * a.block_size)];
+    const int pieces = a.row_bytes / 16, i0 = chunk * EV_ROWS, items = min(EV_ROWS, m - i0) * pieces;
+    for (int w0 = tid; w0 < items; w0 += EV_THREADS * EV_AHEAD) {
+        int64_t src[EV_AHEAD], put[EV_AHEAD], score_src[EV_AHEAD], score_put[EV_AHEAD];   // (put < 0: dropped)
+        u32x4_t k[EV_AHEAD], v[EV_AHEAD];
+        int from[EV_AHEAD], fb[EV_AHEAD], tb[EV_AHEAD];
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) from[u] = kept[i0 + min(w0 + u * EV_THREADS, items - 1) / pieces];
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            fb[u] = table[page_of(a, from[u])];
+            tb[u] = dst[page_of(a, a.prefix_len + i0 + min(w0 + u * EV_THREADS, items - 1) / pieces)];
+        }
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            const int w = min(w0 + u * EV_THREADS, items - 1), off = w % pieces * 16, to = a.prefix_len + i0 + w / pieces;
+            const int fo = from[u] - page_of(a, from[u]) * a.block_size, ro = to - page_of(a, to) * a.block_size;
+            const int f = min(max(fb[u], 0), a.num_blocks - 1);
+            src[u] = f * a.block_stride + ((int64_t)fo * a.Hkv + hk) * a.row_bytes + off;
+            k[u] = *reinterpret_cast<const u32x4_t*>(a.kc + src[u]);
+            v[u] = *reinterpret_cast<const u32x4_t*>(a.vc + src[u]);
+            const bool ok = w0 + u * EV_THREADS < items && tb[u] >= 0 && tb[u] < a.num_blocks;
+            put[u] = ok ? tb[u] * a.block_stride + ((int64_t)ro * a.Hkv + hk) * a.row_bytes + off : -1;
+            score_src[u] = ((int64_t)f * a.Hkv + hk) * a.block_size + fo;
+            score_put[u] = ok && off == 0 ? ((int64_t)tb[u] * a.Hkv + hk) * a.block_size + ro : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            if (put[u] < 0) continue;
+            __builtin_nontemporal_store(k[u], reinterpret_cast<u32x4_t*>(a.kc + put[u]));   // (nobody reads them soon)
+            __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(a.vc + put[u]));
+            if (score_put[u] >= 0) a.scores[score_put[u]] = a.scores[score_src[u]];
+        }
     }
     if (chunk == 0 && m > 0) {   // the rest of the last page
         const int end = a.prefix_len + m, tp = page_of(a, end - 1), tb = dst[tp];

@@ -700,7 +700,6 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
         const float f = join_stats<LANES>(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
         num *= back;
         const int cnt = min(LANES, n - i0);
-#pragma unroll 4
         for (int j = group; j < cnt; j += GROUPS) {
             const float fj = __shfl(f, base + j, 64);
             const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
@@ -724,13 +723,46 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
 constexpr int SA_SCORE_KEYS = 4 * SA_THREADS;
 template <typename E>
 __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int pieces) {
-    constexpr int HEADS = 64;
+    constexpr int HEADS = 64, AHEAD = 8;
     __shared__ float fin[HEADS][2];
     const int hk = id % a.Hkv, piece = id / a.Hkv % pieces, b = id / a.Hkv / pieces, tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ctx = min(a.ctx_lens[b], a.max_ctx), lo = window_lo(a, ctx - 1), first = a.prefix_len + piece * SA_SCORE_KEYS;
     if (first >= ctx || first + SA_SCORE_KEYS <= lo) return;
     const int rel = piece * SA_SCORE_KEYS + 4 * tid;
+    const bool some = a.prefix_len + rel < ctx;
+    const float* x = a.logits + ((int64_t)b * a.Hq + hk * a.G) * a.lstride + rel;
+    // the first heads' logits, the scores so far: on their way while the heads' (m, l) are joined
+    float4_t ahead[AHEAD];
+#pragma unroll
+    for (int g = 0; g < AHEAD; g++)
+        if (some && g < a.G) ahead[g] = *reinterpret_cast<const float4_t*>(x + (int64_t)g * a.lstride);
+    float *slot[4], *slots = nullptr;   // (slots: all four side by side)
+    float old[4];
+    {
+        const int key = a.prefix_len + rel, page = page_of(a, key), off = key - page * a.block_size;
+        if (key + 3 < ctx && key >= lo && off + 3 < a.block_size) {
+            const int blk = a.tables[(int64_t)b * a.max_blocks + page];
+            float* to = a.scores + ((int64_t)min(max(blk, 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + off;
+            if (blk >= 0 && blk < a.num_blocks && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+                slots = to;
+                const float4_t v = *reinterpret_cast<const float4_t*>(to);
+#pragma unroll
+                for (int u = 0; u < 4; u++) old[u] = v[u];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int key = a.prefix_len + rel + u;
+        slot[u] = nullptr;
+        if (slots) continue;
+        if (key >= ctx || key < lo) continue;
+        const int page = page_of(a, key), blk = a.tables[(int64_t)b * a.max_blocks + page];
+        if (blk < 0 || blk >= a.num_blocks) continue;   // no score is written outside the cache
+        slot[u] = a.scores + ((int64_t)blk * a.Hkv + hk) * a.block_size + (key - page * a.block_size);
+        old[u] = *slot[u];
+    }
     float4_t w = {0.f, 0.f, 0.f, 0.f};
     for (int g0 = 0; g0 < a.G; g0 += HEADS) {
         const int heads = min(HEADS, a.G - g0);
@@ -746,24 +778,24 @@ __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int 
             }
         }
         __syncthreads();
-        if (a.prefix_len + rel < ctx) {
-            const float* x = a.logits + ((int64_t)b * a.Hq + hk * a.G + g0) * a.lstride + rel;
-#pragma unroll 4
-            for (int g = 0; g < heads; g++) {
-                const float4_t v = *reinterpret_cast<const float4_t*>(x + (int64_t)g * a.lstride);
+        auto take = [&](float4_t v, int g) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) w[u] += __builtin_amdgcn_exp2f(v[u] - fin[g][0]) * fin[g][1];
-            }
+            for (int u = 0; u < 4; u++) w[u] += __builtin_amdgcn_exp2f(v[u] - fin[g][0]) * fin[g][1];
+        };
+        if (some && g0 == 0) {
+#pragma unroll
+            for (int g = 0; g < AHEAD; g++)
+                if (g < heads) take(ahead[g], g);
+        }
+        if (some) {
+#pragma unroll 4
+            for (int g = g0 ? 0 : AHEAD; g < heads; g++) take(*reinterpret_cast<const float4_t*>(x + (int64_t)(g0 + g) * a.lstride), g);
         }
     }
+    if (slots) *reinterpret_cast<float4_t*>(slots) = float4_t{old[0], old[1], old[2], old[3]} + w;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int key = a.prefix_len + rel + u;
-        if (key >= ctx || key < lo) continue;
-        const int page = page_of(a, key), blk = a.tables[(int64_t)b * a.max_blocks + page];
-        if (blk < 0 || blk >= a.num_blocks) continue;   // no score is written outside the cache
-        a.scores[((int64_t)blk * a.Hkv + hk) * a.block_size + (key - page * a.block_size)] += w[u];
-    }
+    for (int u = 0; u < 4; u++)
+        if (slot[u]) *slot[u] = old[u] + w[u];
 }
 
 template <typename E, int D, int LANES>
