@@ -700,10 +700,11 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
         const float f = join_stats<LANES>(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
         num *= back;
         const int cnt = min(LANES, n - i0);
-        for (int j = group; j < cnt; j += GROUPS) {
+        for (int j0 = 0; j0 < cnt; j0 += GROUPS) {   // (all lanes go along: any of them may be asked for its factor)
+            const int j = min(j0 + group, cnt - 1);
             const float fj = __shfl(f, base + j, 64);
             const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
-            if (fj != 0.f) num += fj * v;   // (what was not written may be anything)
+            if (j0 + group < cnt && fj != 0.f) num += fj * v;   // (what was not written may be anything)
         }
     }
 #pragma unroll

@@ -113,6 +113,8 @@ LAYOUTS = [(64, 8, 64, F16), (8, 2, 128, BF16), (6, 2, 64, BF16), (5, 1, 128, F1
 DECODE = [
     ([1], 0, 16, 0, False), ([1, 2, 33], 0, 16, 0, True), ([31, 32, 33, 64, 65], 7, 16, 0, False), ([1, 300], 257, 20, 0, True),
     ([5, 1, 17], 1000, 16, 0, True), ([1, 9], 1, 1, 0, False), ([130, 1, 4], 333, 48, 128, True), ([1, 40], 64, 16, 1, False),
+    ([1], 2048, 16, 0, True), ([130], 2050, 16, 0, False), ([1], 4096, 32, 0, False), ([1], 8192, 64, 0, True), ([1, 2], 2300, 16, 0, True), ([3], 5800, 16, 0, True),
+    # (the line above: 17 to 65 ranges, also numbers of them that a wave's lane groups do not divide)
     ([2, 700, 90], 31, 128, 600, False), ([0, 3, 0], 50, 16, 0, False), ([1, 2], 300, 16, 5, True),
 ]
 
