@@ -684,6 +684,7 @@ __device__ __forceinline__ float inverse(float den) { return den > 0.f ? 1.0f / 
 template <typename E, int D, int LANES>
 __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
     constexpr int LPR = D / 4, GROUPS = LANES / LPR, ROWS = SA_THREADS / LANES;
+    constexpr int AHEAD = LANES == 64 ? 8 : 4;   // ranges whose rows are requested at a time
     const int lane = threadIdx.x % LANES, base = (threadIdx.x & 63) - lane, group = lane / LPR, col = lane % LPR * 4;
     const int hk = id % a.Hkv, row_asked = id / a.Hkv * ROWS + (int)threadIdx.x / LANES;   // (a KV head's rows stay on their chiplet)
     const int row = min(row_asked, a.T * a.G - 1);
@@ -700,11 +701,22 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
         const float f = join_stats<LANES>(range_stat(a, i0 + lane, r, pos, lo), m_run, den, back);
         num *= back;
         const int cnt = min(LANES, n - i0);
-        for (int j0 = 0; j0 < cnt; j0 += GROUPS) {   // (all lanes go along: any of them may be asked for its factor)
-            const int j = min(j0 + group, cnt - 1);
-            const float fj = __shfl(f, base + j, 64);
-            const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + j) * rows + r) * D + col);
-            if (j0 + group < cnt && fj != 0.f) num += fj * v;   // (what was not written may be anything)
+        auto take = [&](auto ahead, int j0) {   // (all lanes go along: any of them may be asked for its factor)
+            constexpr int N = decltype(ahead)::value;
+            float4_t v[N];
+#pragma unroll
+            for (int u = 0; u < N; u++)
+                v[u] = *reinterpret_cast<const float4_t*>(a.part_o + ((i0 + min(j0 + u * GROUPS + group, cnt - 1)) * rows + r) * D + col);
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const int j = j0 + u * GROUPS + group;
+                const float fj = __shfl(f, base + min(j, cnt - 1), 64);
+                if (j < cnt && fj != 0.f) num += fj * v[u];   // (what was not written may be anything)
+            }
+        };
+        for (int j0 = 0; j0 < cnt; j0 += AHEAD * GROUPS) {
+            if (cnt - j0 > 2 * GROUPS) take(std::integral_constant<int, AHEAD>{}, j0);
+            else take(std::integral_constant<int, 2>{}, j0);
         }
     }
 #pragma unroll
@@ -809,20 +821,28 @@ __global__ __launch_bounds__(SA_THREADS) void shared_join_kernel(SharedAttnArgs 
 // Into how many ranges a walk over `keys` keys is cut, for `units` (row set, KV head) pairs.  More ranges fill the 256 CUs
 // and even them out; each costs its workgroups' start and the writing and reading of its rows' outputs.  In ns, fitted to
 // sweeps of 1 to 64 ranges over prefixes of 8192 and 20011 keys, 32 to 2500 tokens, and own contexts of 512 to 65536:
-//   7000 + len * max(alone, share * c) + 1300 c + merge * n     c: workgroups per CU, whole ones until there are four
+//   7000 + len * max(alone, share * c) + start * c + merge * n + uneven   c: workgroups per CU, whole ones until there are four
 // alone: ns per key of one workgroup on a CU, share: of all of a CU's workgroups together.  A few workgroups over a whole
 // number per CU cost arithmetic (`tiles`) little, memory another round.  `beside`: time of memory-bound work of the same
-// launch, which runs in the shadow of one workgroup per CU, but behind a second one.
-static void cut_keys(int64_t keys, int64_t units, bool tiles, double alone, double share, double merge, double beside, int& n, int& len) {
+// launch, which runs in the shadow of one workgroup per CU, but behind a second one.  uneven = 0.4 * alone * len / c for own
+// tokens, whose sequences differ in length: on a CU with few long ranges, the prefix's (`others`) among them, their sums differ
+// more (8 sequences of 500 to 65536 tokens, D 128: 16 ranges 153 us, 32 ranges 118; 32 of 1000 to 4096: 2 ranges 73 us, 4
+// ranges 71.5; but 64 of up to 1024: 1 range 34 us, 2 ranges 37).
+struct CutCost {
+    bool tiles;
+    double alone, share, start, uneven, merge, beside, others;
+};
+static void cut_keys(int64_t keys, int64_t units, const CutCost& w, int& n, int& len) {
     n = 0, len = 128;
     if (keys <= 0) return;
     double best = 0;
     for (int64_t k = 1; k <= 1024 && (k == 1 || (k - 1) * 128 < keys); k += k < 16 ? 1 : k / 8) {
         const int64_t l = ((keys + k - 1) / k + 127) / 128 * 128, used = (keys + l - 1) / l;
-        const double c = (double)(units * used) / 256, whole = c <= 1 ? 1 : c < 4 ? ceil(c - (tiles ? 0.125 : 0)) : c;
-        const double per_key = share * whole;
+        const double c = (double)(units * used) / 256, whole = c <= 1 ? 1 : c < 4 ? ceil(c - (w.tiles ? 0.125 : 0)) : c;
+        const double per_key = w.share * whole;
         const double behind = c <= 1 ? 0 : c < 2 ? c - 1 : 1;
-        const double t = 7000 + l * (per_key > alone ? per_key : alone) + 1300 * c + merge * used + 0.5 * behind * beside;
+        const double t = 7000 + l * (per_key > w.alone ? per_key : w.alone) + w.start * c + w.merge * used +
+                         w.uneven * w.alone * l / (c + w.others < 1 ? 1 : c + w.others) + 0.5 * behind * w.beside;
         if (n == 0 || t < best) best = t, n = (int)used, len = (int)l;
     }
 }
@@ -838,15 +858,19 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
     p.prefix_rows = R <= 32 ? 32 : D == 64 && R * Hkv >= 32768 && !scored ? 256 : 128;
     p.own_rows = max_q * G > 32 && !scored ? 128 : 32;
-    const double merge = (double)T * Hq * D * 4 / 2500, wide = D / 64;
-    auto cut = [&](int64_t keys, int64_t units, int rows, double beside, int& n, int& len) {
-        if (rows == 32) cut_keys(keys, units, false, 14 * wide, 13 * wide, merge, beside, n, len);
-        else if (rows == 128) cut_keys(keys, units, true, wide == 1 ? 18 : 33, wide == 1 ? 11.2 : 20, merge, beside, n, len);
-        else cut_keys(keys, units, true, 36, 21.7, merge, beside, n, len);
+    const double merge = (double)T * Hq * D * 4 / 2500;
+    const bool d64 = D <= 64;
+    const int64_t prefix_units = Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows);
+    auto cut = [&](bool own_keys, int rows, int64_t keys, int64_t units, double beside, int& n, int& len) {
+        CutCost w{true, 36, 21.7, 1300, 0, merge, beside, 0};                      // 256 rows
+        if (rows == 128) w.alone = d64 ? 18 : 33, w.share = d64 ? 11.2 : 20;
+        if (rows == 32) w.tiles = false, w.alone = d64 ? 14 : 28, w.share = d64 ? 13 : 26;
+        if (rows == 32 && own_keys) w.start = d64 ? 1300 : 4000, w.uneven = 0.4, w.others = (double)p.np * prefix_units / 256;
+        cut_keys(keys, units, w, n, len);
     };
-    cut(P, Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows), p.prefix_rows,
+    cut(false, p.prefix_rows, P, prefix_units,
         p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0, p.np, p.sp);
-    cut(own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), p.own_rows, 0, p.ns, p.so);
+    cut(true, p.own_rows, own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), 0, p.ns, p.so);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)((own + 127) / 128 * 128);
