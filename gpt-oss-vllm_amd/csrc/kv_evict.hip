@@ -135,9 +135,9 @@ __device__ __forceinline__ int lanes_below(uint64_t votes) {
 
 // Lists in order the candidates above `limit` and the first `left` equal to it.  Each wave looks after a run of consecutive
 // tokens, 64 of them at a time, so that positions come out in order from ballots alone; each(f) calls f(token, above, equal)
-// for the wave's steps.
+// for the wave's steps.  Nothing is written behind entry c, whatever another stream does to the scores between the passes.
 template <int THREADS, typename EACH>
-__device__ __forceinline__ void list_kept(const EvictArgs& a, int32_t* kept, int left, EACH each) {
+__device__ __forceinline__ void list_kept(const EvictArgs& a, int32_t* kept, int c, int left, EACH each) {
     __shared__ int wave_gt[THREADS / 64], wave_eq[THREADS / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int gt = 0, eq = 0;
@@ -161,7 +161,7 @@ __device__ __forceinline__ void list_kept(const EvictArgs& a, int32_t* kept, int
         const bool take = above || (equal && seen + lanes_below(eqs) < left);
         seen += __popcll(eqs);
         const uint64_t takes = __ballot(take);
-        if (take) kept[at + lanes_below(takes)] = a.prefix_len + i;
+        if (take && at + lanes_below(takes) < c) kept[at + lanes_below(takes)] = a.prefix_len + i;
         at += __popcll(takes);
     });
 }
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
     });
     __syncthreads();
     limit = limit << 10 | find_bin<THREADS, 1024>(hist, left);
-    list_kept<THREADS>(a, s.kept, left, [&](auto f) { each([&](int i, uint32_t k, bool in) { f(i, in && k > limit, in && k == limit); }); });
+    list_kept<THREADS>(a, s.kept, s.c, left, [&](auto f) { each([&](int i, uint32_t k, bool in) { f(i, in && k > limit, in && k == limit); }); });
 }
 
 // Exclusive prefix sum over the wave, and its total.
@@ -397,10 +397,13 @@ __global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
             seen += total;
         }
         int total;
-        int32_t* to = s.kept + at + wave_scan(__popc(above), total);
+        int to = at + wave_scan(__popc(above), total);
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            if (above >> e & 1) *to++ = a.prefix_len + i + e;
+            if (above >> e & 1) {
+                if (to < s.c) s.kept[to] = a.prefix_len + i + e;   // (see list_kept)
+                to++;
+            }
         at += total;
     });
 }
@@ -419,7 +422,8 @@ __global__ __launch_bounds__(EV_THREADS) void kv_move_kernel(EvictArgs a, int ch
         u32x4_t k[EV_AHEAD], v[EV_AHEAD];
         int from[EV_AHEAD], fb[EV_AHEAD], tb[EV_AHEAD];
 #pragma unroll
-        for (int u = 0; u < EV_AHEAD; u++) from[u] = kept[i0 + min(w0 + u * EV_THREADS, items - 1) / pieces];
+        for (int u = 0; u < EV_AHEAD; u++)   // (clamped: no access leaves the table, whatever became of the scores)
+            from[u] = min(max(kept[i0 + min(w0 + u * EV_THREADS, items - 1) / pieces], 0), a.max_ctx - 1);
 #pragma unroll
         for (int u = 0; u < EV_AHEAD; u++) {
             fb[u] = table[page_of(a, from[u])];
