@@ -44,6 +44,8 @@ struct SharedAttnArgs {
     int page_shift;
     int64_t block_stride, q_stride, o_stride;
     int prefix_len, max_ctx, max_q, window;
+    int folded;                                  // prefix tokens that the own walks take along (prefix_len is then 0)
+    int direct;                                  // one range in all: its workgroups write the output themselves
     float scale2;                                // |scale| * log2(e): scores are in the units of exp2
     uint32_t q_sign;                             // flips q's signs when scale is negative
     int np, sp, ns, so;                          // ranges over the prefix / the own tokens, and their lengths
@@ -197,6 +199,59 @@ __device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t a2, u
         : "memory");
 }
 
+// The ranges of one row, lane i looking after range i0 + i: does the row see a key of it (else nothing was written), and
+// its (m, l).
+struct RangeStat {
+    bool live;
+    float m, l;
+};
+__device__ __forceinline__ RangeStat range_stat(const SharedAttnArgs& a, int i, int64_t r, int pos, int lo) {
+    const int beg = i < a.np ? i * a.sp : a.prefix_len + (i - a.np) * a.so;
+    const int end = i < a.np ? min(beg + a.sp, a.prefix_len) : beg + a.so;
+    RangeStat s{i < a.np + a.ns && max(beg, lo) < min(end, pos + 1), SA_NONE, 0.f};
+    if (s.live) {
+        const float* ml = a.part_ml + (i * (int64_t)a.T * a.Hq + r) * 2;
+        s.m = ml[0];
+        s.l = ml[1];
+    }
+    return s;
+}
+template <typename E>
+__device__ __forceinline__ void start_with_sink(const SharedAttnArgs& a, int head, float& m, float& den) {
+    m = SA_NONE;
+    den = 0.f;
+    if (a.sinks) {   // one more logit in the denominator
+        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
+        m = sk > SA_NONE ? sk : SA_NONE;
+        den = sk == -INFINITY ? 0.f : sk == sk ? 1.0f : sk;   // (a NaN stays one)
+    }
+}
+// One step of the running (m, den) over the ranges of N neighbouring lanes: returns this lane's factor (0: leave its range
+// out).
+template <int N>
+__device__ __forceinline__ float join_stats(const RangeStat& s, float& m_run, float& den, float& back) {
+    float top = s.m;
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float m_new = fmaxf(m_run, top);
+    back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+    const float f = !s.live || s.l == 0.f ? 0.f : s.m == m_new ? 1.0f : __builtin_amdgcn_exp2f(s.m - m_new);
+    float part = f == 0.f && s.l == s.l ? 0.f : f * s.l;
+#pragma unroll
+    for (int o = 1; o < N; o *= 2) part += __shfl_xor(part, o, 64);
+    den = den * back + part;
+    m_run = m_new;
+    return f;
+}
+__device__ __forceinline__ float inverse(float den) { return den > 0.f ? 1.0f / den : den == 0.f ? 0.f : den; }
+// Four columns of a row's output (of any alignment).
+template <typename E>
+__device__ __forceinline__ void put_out(const SharedAttnArgs& a, int token, int head, int D, int c, float4_t num, float inv) {
+    E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + 4 * c;
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = (E)(num[i] * inv);
+}
+
 // Shape of a workgroup's walk.  RW = 4: every wave holds 32 * QT rows, tiles of 64 keys are shared, NS of them in LDS or on
 // their way.  RW = 1: one set of 32 rows, the waves take tiles of 32 keys in turn, each in LDS of its own; a tile is read
 // into registers whole, and the next one requested into its place before the softmax.
@@ -210,27 +265,35 @@ struct Walk {
     static constexpr int LDS = TILES + SA_WAVES * SA_PAGES * 4;              // and every wave's slice of the page table
 };
 
-// A wave's slice of the page table from page `from` on.  Entries behind the row's end repeat its last one, and an entry
-// outside the cache is clamped: no access leaves either, whatever the table holds.
+// The pages of a walk as one list: those of the first `folded` tokens from row 0 of the block tables, then the row's own from
+// the page of token `folded` on (which is a second entry for that page if the folded tokens end inside it).
+__device__ __forceinline__ int split_page(const SharedAttnArgs& a, int folded) { return folded > page_of(a, folded) * a.block_size ? 1 : 0; }
+// A wave's slice of that list from entry `from` on.  Entries behind the row's end repeat its last one, and an entry outside
+// the cache is clamped: no access leaves either, whatever the table holds.
 template <int D, int RW>
-__device__ __forceinline__ void fetch_pages(const SharedAttnArgs& a, unsigned char* smem, const int32_t* table, int from) {
+__device__ __forceinline__ void fetch_pages(const SharedAttnArgs& a, unsigned char* smem, const int32_t* table, int from, int folded) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int32_t* pages = reinterpret_cast<int32_t*>(smem + Walk<D, RW>::TILES) + wave * SA_PAGES;
+    const int extra = split_page(a, folded), shared_pages = page_of(a, folded) + extra;
     int raw[SA_PAGES / 64];
 #pragma unroll
-    for (int i = 0; i < SA_PAGES / 64; i++) raw[i] = table[min(from + 64 * i + lane, a.max_blocks - 1)];
+    for (int i = 0; i < SA_PAGES / 64; i++) {
+        const int entry = from + 64 * i + lane;
+        raw[i] = entry < shared_pages ? a.tables[min(entry, a.max_blocks - 1)] : table[min(entry - extra, a.max_blocks - 1)];
+    }
 #pragma unroll
     for (int i = 0; i < SA_PAGES / 64; i++) pages[64 * i + lane] = min(max(raw[i], 0), a.num_blocks - 1);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // One workgroup: the rows [row0, row_end) of KV head hk (at most 32 * RW * QT) over the keys [kbeg, kend) of `table`, of
-// which those from kfloor on may be read.  pos / lo: position and lowest visible key of this lane's row(s).  The waves' table
-// slices hold the entries from pages_from on (fetch_pages).
+// which those from kfloor on may be read, the first `folded` through row 0.  pos / lo: position and lowest visible key of this
+// lane's row(s).  The waves' slices of the page list start with entry pages_from (fetch_pages).  direct: no other range has keys
+// of these rows, so the output is written here.
 template <typename E, int D, int RW, int QT, bool SCORED>
 __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* smem, int hk, int row0, int row_end, const int (&pos)[QT],
                                        const int (&lo)[QT], const int32_t* table, int pages_from, int kbeg, int kend, int kfloor,
-                                       int split, int own_b, int own_k0) {
+                                       int split, int own_b, int own_k0, int folded, bool direct) {
     typedef Walk<D, RW> W;
     constexpr int KT = W::KT, ROW = D * 2, STEPS = D / 16, DT = D / 32, NI = W::NI, AHEAD = RW == 1 ? 1 : W::NS - 1;
     constexpr int VH = RW == 4 && DT == 4 ? 1 : 2;   // V fragments of how many 16-key halves are held at a time
@@ -267,14 +330,16 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
     const int32_t* pages = reinterpret_cast<const int32_t*>(smem + W::TILES) + wave * SA_PAGES;
     // keys outside re-read the nearest one: they are masked below, and rows nobody may see are never read
     auto readable = [&](int key) { return max(min(key, kend - 1), kfloor); };
+    const int extra = split_page(a, folded);
+    auto entry_of = [&](int key) { return page_of(a, key) + (key >= folded ? extra : 0); };
     auto stage = [&](int t) {
         const int k_first = key_of(t);
-        if (page_of(a, readable(k_first + KT - 1)) >= pages_from + SA_PAGES) {   // (uniform; a tile spans at most KT < SA_PAGES pages)
-            pages_from = page_of(a, readable(k_first));
-            fetch_pages<D, RW>(a, smem, table, pages_from);
+        if (entry_of(readable(k_first + KT - 1)) >= pages_from + SA_PAGES) {   // (uniform; a tile spans at most KT + 1 < SA_PAGES pages)
+            pages_from = entry_of(readable(k_first));
+            fetch_pages<D, RW>(a, smem, table, pages_from, folded);
         }
         const int key = readable(k_first + (lane & (KT - 1))), page = page_of(a, key);   // lane l looks up key l
-        const int64_t off = pages[page - pages_from] * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D;
+        const int64_t off = pages[entry_of(key) - pages_from] * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D;
         unsigned char* dst = tiles + (t % W::NS) * W::STAGE + (RW == 4 ? wave * NI * 1024 : 0);
         int64_t src[NI];
 #pragma unroll
@@ -507,6 +572,20 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             const float l = half_sum(l_run[q]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const int first = row0 + 32 * (wave * QT + q), c = lane % CH;
+            if (direct) {
+                float m, den, back;
+                start_with_sink<E>(a, head[q], m, den);
+                const float f = join_stats<1>(RangeStat{true, m_run[q], l}, m, den, back), inv = inverse(den);
+#pragma unroll
+                for (int i = 0; i < 32 * CH / 64; i++) {
+                    const int r32 = i * (64 / CH) + lane / CH, rr = first + r32;
+                    const float fr = __shfl(f, r32, 64), ir = __shfl(inv, r32, 64);
+                    const float4_t v = get(at, r32, c);
+                    if (rr < row_end) put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, fr != 0.f ? fr * v : float4_t{0.f, 0.f, 0.f, 0.f}, ir);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < 32 * CH / 64; i++) {
                 const int r32 = i * (64 / CH) + lane / CH, rr = first + r32;
@@ -545,6 +624,13 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                 l += f * wl[w][r32];
             }
             const int rr = row0 + r32;
+            if (direct) {
+                float m_all, den, back;
+                start_with_sink<E>(a, hk * a.G + rr % a.G, m_all, den);
+                const float f = join_stats<1>(RangeStat{true, m, l}, m_all, den, back);
+                put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, f != 0.f ? f * tot : float4_t{0.f, 0.f, 0.f, 0.f}, inverse(den));
+                continue;
+            }
             const int64_t r = split * rows + (int64_t)(rr / a.G) * a.Hq + hk * a.G + rr % a.G;
             *reinterpret_cast<float4_t*>(a.part_o + r * D + 4 * c) = tot;
             if (c == 0) {
@@ -562,7 +648,7 @@ __device__ __forceinline__ void prefix_part(const SharedAttnArgs& a, unsigned ch
     __shared__ int ends[SA_WAVES][2];
     const int hk = id % a.Hkv, unit = id / a.Hkv, split = unit % a.np, row0 = unit / a.np * ROWS;
     const int row_end = min(a.T * a.G, row0 + ROWS), pages_from = page_of(a, split * a.sp);
-    fetch_pages<D, RW>(a, smem, a.tables, pages_from);   // (needs nothing that is still to be looked up)
+    fetch_pages<D, RW>(a, smem, a.tables, pages_from, 0);   // (needs nothing that is still to be looked up)
     const int tid = threadIdx.x, wave = tid >> 6, qi = tid & 31;
     int pos[QT], lo[QT], pos_max = -1, lo_min = INT32_MAX;
 #pragma unroll
@@ -593,7 +679,7 @@ __device__ __forceinline__ void prefix_part(const SharedAttnArgs& a, unsigned ch
     }
     const int kbeg = max(split * a.sp, lo_min), kend = min(min(split * a.sp + a.sp, a.prefix_len), pos_max + 1);
     if (kbeg >= kend) return;   // (the merge leaves out a range that a row does not see)
-    attend<E, D, RW, QT, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables, pages_from, kbeg, kend, kbeg, split, 0, -1);
+    attend<E, D, RW, QT, SCORED>(a, smem, hk, row0, row_end, pos, lo, a.tables, pages_from, kbeg, kend, kbeg, split, 0, -1, 0, false);
 }
 
 // The sequences' own tokens: a workgroup per (sequence, row set of the longest sequence, range, KV head).
@@ -602,22 +688,25 @@ __device__ __forceinline__ void own_part(const SharedAttnArgs& a, unsigned char*
     const int hk = id % a.Hkv, unit = id / a.Hkv, split = unit % a.ns;
     const int b = unit / a.ns / row_sets, set = unit / a.ns % row_sets;
     const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    const int k0 = a.prefix_len + split * a.so, pages_from = page_of(a, k0);
-    fetch_pages<D, RW>(a, smem, table, pages_from);
+    const int k0 = a.prefix_len + split * a.so, folded = SCORED ? 0 : a.folded;
+    const int pages_from = page_of(a, k0) + (k0 >= folded ? split_page(a, folded) : 0);
+    fetch_pages<D, RW>(a, smem, table, pages_from, folded);
     const SeqSpan s = seq_span(a, b);
-    const int row0 = s.t0 * a.G + set * 32 * RW, row_end = min((s.t0 + s.n) * a.G, row0 + 32 * RW);
+    const int row0 = s.t0 * a.G + set * 32 * RW, row_end = min((s.t0 + min(s.n, a.max_q)) * a.G, row0 + 32 * RW);
     if (row0 >= row_end) return;
     const int tid = threadIdx.x, wave = tid >> 6, qi = tid & 31;
     const int row = min(row0 + (RW == 4 ? 32 * wave : 0) + qi, row_end - 1);
     const int pos0 = s.ctx - s.n - s.t0;                       // position of token t is pos0 + t
     const int pos[1] = {pos0 + row / a.G}, lo[1] = {window_lo(a, pos[0])};
     const int kbeg = max(k0, window_lo(a, pos0 + row0 / a.G));
-    const int kend = min(k0 + a.so, pos0 + (row_end - 1) / a.G + 1);
-    if (kbeg >= kend) return;
+    int kend = min(k0 + a.so, pos0 + (row_end - 1) / a.G + 1);
+    const bool direct = !SCORED && a.direct;
+    if (kbeg >= kend && !direct) return;
+    kend = max(kend, kbeg);   // (direct: rows that see nothing are written all the same)
     // (scored: the logits are addressed from the range's start in steps of a tile, so the walk starts on one)
     const int start = SCORED ? k0 + (kbeg - k0) / 32 * 32 : kbeg;
     attend<E, D, RW, 1, SCORED>(a, smem, hk, row0, row_end, pos, lo, table, pages_from, start, kend, kbeg, a.np + split, b,
-                                SCORED ? a.prefix_len : -1);
+                                SCORED ? a.prefix_len : -1, folded, direct);
 }
 
 // Both in one launch: the prefix (bound by the matrix cores when there are many rows) and the own tokens (bound by memory)
@@ -629,52 +718,6 @@ __global__ __launch_bounds__(SA_THREADS, D == 64 && QT == 1 ? 3 : 2) void shared
     if ((int)blockIdx.x < prefix_wgs) prefix_part<E, D, RWP, QT, SCORED>(a, smem, blockIdx.x);
     else own_part<E, D, RWO, SCORED>(a, smem, blockIdx.x - prefix_wgs, row_sets);
 }
-
-// The ranges of one row, lane i looking after range i0 + i: does the row see a key of it (else nothing was written), and
-// its (m, l).
-struct RangeStat {
-    bool live;
-    float m, l;
-};
-__device__ __forceinline__ RangeStat range_stat(const SharedAttnArgs& a, int i, int64_t r, int pos, int lo) {
-    const int beg = i < a.np ? i * a.sp : a.prefix_len + (i - a.np) * a.so;
-    const int end = i < a.np ? min(beg + a.sp, a.prefix_len) : beg + a.so;
-    RangeStat s{i < a.np + a.ns && max(beg, lo) < min(end, pos + 1), SA_NONE, 0.f};
-    if (s.live) {
-        const float* ml = a.part_ml + (i * (int64_t)a.T * a.Hq + r) * 2;
-        s.m = ml[0];
-        s.l = ml[1];
-    }
-    return s;
-}
-template <typename E>
-__device__ __forceinline__ void start_with_sink(const SharedAttnArgs& a, int head, float& m, float& den) {
-    m = SA_NONE;
-    den = 0.f;
-    if (a.sinks) {   // one more logit in the denominator
-        const float sk = (float)reinterpret_cast<const E*>(a.sinks)[head] * 1.44269504088896341f;
-        m = sk > SA_NONE ? sk : SA_NONE;
-        den = sk == -INFINITY ? 0.f : sk == sk ? 1.0f : sk;   // (a NaN stays one)
-    }
-}
-// One step of the running (m, den) over the ranges of N neighbouring lanes: returns this lane's factor (0: leave its range
-// out).
-template <int N>
-__device__ __forceinline__ float join_stats(const RangeStat& s, float& m_run, float& den, float& back) {
-    float top = s.m;
-#pragma unroll
-    for (int o = 1; o < N; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float m_new = fmaxf(m_run, top);
-    back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-    const float f = !s.live || s.l == 0.f ? 0.f : s.m == m_new ? 1.0f : __builtin_amdgcn_exp2f(s.m - m_new);
-    float part = f == 0.f && s.l == s.l ? 0.f : f * s.l;
-#pragma unroll
-    for (int o = 1; o < N; o *= 2) part += __shfl_xor(part, o, 64);
-    den = den * back + part;
-    m_run = m_new;
-    return f;
-}
-__device__ __forceinline__ float inverse(float den) { return den > 0.f ? 1.0f / den : den == 0.f ? 0.f : den; }
 
 // Joins a row's ranges, LANES lanes per (token, query head): each looks after one range's (m, l), then they take the ranges'
 // outputs on, D / 4 lanes to a range's row.  LANES = 64: a wave's whole width on one row, LANES / (D / 4) ranges at a time,
@@ -725,10 +768,7 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
         for (int c = 0; c < 4; c++) num[c] += __shfl_xor(num[c], st, 64);
     // rows behind the last sequence, and tokens behind the longest one that was announced, leave the output as it was
     if (group || row_asked >= a.T * a.G || b < 0 || token - s.t0 >= a.max_q) return;
-    const float inv = inverse(den);
-    E* out = reinterpret_cast<E*>(a.out) + token * a.o_stride + head * D + col;
-#pragma unroll
-    for (int c = 0; c < 4; c++) out[c] = (E)(num[c] * inv);
+    put_out<E>(a, token, head, D, lane % LPR, num, inverse(den));
 }
 
 // Adds the own tokens' weights, summed over the group's query heads: a workgroup per (sequence, KV head, SA_SCORE_KEYS
@@ -832,27 +872,34 @@ struct CutCost {
     bool tiles;
     double alone, share, start, uneven, merge, beside, others;
 };
-static void cut_keys(int64_t keys, int64_t units, const CutCost& w, int& n, int& len) {
+// Cost of ranges of `len` keys.
+static double cut_cost(int64_t keys, int64_t units, const CutCost& w, int64_t len) {
+    const int64_t used = (keys + len - 1) / len;
+    const double c = (double)(units * used) / 256, whole = c <= 1 ? 1 : c < 4 ? ceil(c - (w.tiles ? 0.125 : 0)) : c;
+    const double per_key = w.share * whole;
+    const double behind = c <= 1 ? 0 : c < 2 ? c - 1 : 1;
+    return 7000 + len * (per_key > w.alone ? per_key : w.alone) + w.start * c + w.merge * used +
+           w.uneven * w.alone * len / (c + w.others < 1 ? 1 : c + w.others) + 0.5 * behind * w.beside;
+}
+static double cut_keys(int64_t keys, int64_t units, const CutCost& w, int& n, int& len) {
     n = 0, len = 128;
-    if (keys <= 0) return;
+    if (keys <= 0) return 0;
     double best = 0;
     for (int64_t k = 1; k <= 1024 && (k == 1 || (k - 1) * 128 < keys); k += k < 16 ? 1 : k / 8) {
-        const int64_t l = ((keys + k - 1) / k + 127) / 128 * 128, used = (keys + l - 1) / l;
-        const double c = (double)(units * used) / 256, whole = c <= 1 ? 1 : c < 4 ? ceil(c - (w.tiles ? 0.125 : 0)) : c;
-        const double per_key = w.share * whole;
-        const double behind = c <= 1 ? 0 : c < 2 ? c - 1 : 1;
-        const double t = 7000 + l * (per_key > w.alone ? per_key : w.alone) + w.start * c + w.merge * used +
-                         w.uneven * w.alone * l / (c + w.others < 1 ? 1 : c + w.others) + 0.5 * behind * w.beside;
-        if (n == 0 || t < best) best = t, n = (int)used, len = (int)l;
+        const int64_t l = ((keys + k - 1) / k + 127) / 128 * 128;
+        const double t = cut_cost(keys, units, w, l);
+        if (n == 0 || t < best) best = t, n = (int)((keys + l - 1) / l), len = (int)l;
     }
+    return best;
 }
 struct SharedAttnPlan {
     int np, sp, ns, so, lstride;
+    bool direct;                 // one range, which takes the prefix along
     int prefix_rows, own_rows;   // rows per workgroup: 32 (RW = 1), 128 or 256 (RW = 4)
     int64_t units;               // an upper bound of every launch's workgroups and row numbers
     size_t part_floats, logit_floats, bytes;
 };
-static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, bool scored) {
+static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, int window, bool scored) {
     SharedAttnPlan p;
     max_q = max_q < T ? max_q : T;
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
@@ -861,21 +908,41 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     const double merge = (double)T * Hq * D * 4 / 2500;
     const bool d64 = D <= 64;
     const int64_t prefix_units = Hkv * ((R + p.prefix_rows - 1) / p.prefix_rows);
-    auto cut = [&](bool own_keys, int rows, int64_t keys, int64_t units, double beside, int& n, int& len) {
-        CutCost w{true, 36, 21.7, 1300, 0, merge, beside, 0};                      // 256 rows
+    auto cost = [&](bool own_keys, int rows, double beside) {
+        CutCost w{true, 36, 21.7, 1300, 0, merge, beside, 0};                   // 256 rows
         if (rows == 128) w.alone = d64 ? 18 : 33, w.share = d64 ? 11.2 : 20;
         if (rows == 32) w.tiles = false, w.alone = d64 ? 14 : 28, w.share = d64 ? 13 : 26;
         if (rows == 32 && own_keys) w.start = d64 ? 1300 : 4000, w.uneven = 0.4, w.others = (double)p.np * prefix_units / 256;
-        cut_keys(keys, units, w, n, len);
+        return w;
     };
-    cut(false, p.prefix_rows, P, prefix_units,
-        p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0, p.np, p.sp);
-    cut(true, p.own_rows, own, Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows), 0, p.ns, p.so);
+    const int64_t own_units = Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows);
+    double t = cut_keys(P, prefix_units, cost(false, p.prefix_rows, p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0), p.np, p.sp);
+    t += cut_keys(own, own_units, cost(true, p.own_rows, 0), p.ns, p.so) - (P && own > 0 ? 7000 : 0);
+    // One range per sequence, which takes the prefix along, instead: every sequence reads the prefix again (from the L2s), but
+    // no outputs are left to be joined, nor is there a second launch (2500 ns of the host's time, and a base of 5500 for 7000).
+    // Fitted to 31 pairs, among them (us of kernels, ranges and joining / one range): 4 sequences of 200 + 33 tokens 9.6 / 7.2,
+    // 16 of 500 + 100 13.1 / 9.5, 32 of 1500 + 60 14.7 / 15.7, 32 of 8192 + 512 22.9 / 58.9; 45 prompts of 42 to 81 tokens
+    // behind 9 92 / 38, 24 of 200 to 300 behind 512 282 / 173, 6 of 150 to 420 behind 8192 364 / 410.
+    auto one_range = [&](int64_t keys_prefix, int64_t keys_own) {
+        CutCost w = cost(true, p.own_rows, 0);
+        const int64_t keys = keys_prefix + keys_own;
+        w.merge = w.others = 0;
+        const double uneven = p.own_rows == 32 ? w.uneven * w.alone * keys_own : 0, c = (double)own_units / 256;
+        if (p.own_rows == 32) w.alone = d64 ? 6 : 10, w.share = (w.alone * keys_prefix + w.share * keys_own) / keys;
+        w.uneven = 0;
+        return cut_cost(keys, own_units, w, (keys + 127) / 128 * 128) + uneven / (c < 1 ? 1 : c) - (p.own_rows == 32 ? 1500 : 0);
+    };
+    p.direct = !scored && one_range(P, own) < t + 2500;
+    if (p.direct) p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)((own + 127) / 128 * 128);
     p.logit_floats = scored ? rows * (size_t)p.lstride : 0;
     p.bytes = (p.part_floats + p.logit_floats) * sizeof(float);
+    if (window > 0 && !scored && !p.direct) {   // (a row set sees its queries' positions and the window in front of the first)
+        const int64_t seen = (int64_t)window + (p.own_rows == 32 ? max_q : 128 / G + 1);
+        if (seen < max_ctx && one_range(0, seen) < t + 2500) p.direct = true, p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
+    }
     p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_SCORE_KEYS + 1);
     return p;
 }
@@ -898,6 +965,7 @@ static int launch_shared_attn(SharedAttnArgs& a, const SharedAttnPlan& p, bool s
         M355_LAUNCH_CHECK("shared_attn_kernel");
     }
 #undef M355_SA
+    if (a.direct) return 0;
     const bool many = (int64_t)rows * a.Hkv > 16384;   // twice the waves that the chip holds at once
     const int per = SA_THREADS / (many ? D / 4 : 64), merge_wgs = a.Hkv * ((rows + per - 1) / per);
     const int pieces = scored ? (a.max_ctx - a.prefix_len + SA_SCORE_KEYS - 1) / SA_SCORE_KEYS : 0, join_grid = merge_wgs + a.Hkv * a.B * pieces;
@@ -928,7 +996,7 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     if (q_stride < (int64_t)Hq * D || o_stride < (int64_t)Hq * D || q_stride % 8)
         return fail(-2, "%s: token strides must cover the heads, q's be a multiple of 8 elements", who);
     if (!aligned(q, 16) || !aligned(kc, 16) || !aligned(vc, 16)) return fail(-3, "%s: q and caches must be 16-byte aligned", who);
-    p = plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, scored);
+    p = plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, window, scored);
     if (max_ctx > (1 << 30) || p.units >= (1ll << 30))
         return fail(-2, "%s: unsupported size T=%d B=%d max_q=%d Hq=%d max_ctx=%d", who, T, B, max_q, Hq, max_ctx);
     if (!workspace || ws_bytes < p.bytes) return fail(-6, "%s: workspace of %zu bytes needed, %zu given", who, p.bytes, ws_bytes);
@@ -943,6 +1011,8 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     a.scale2 = fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f);
     a.q_sign = scale < 0.f ? 0x80008000u : 0u;
     a.np = p.np, a.sp = p.sp, a.ns = p.ns, a.so = p.so;
+    a.direct = p.direct;
+    if (p.direct) a.folded = a.prefix_len, a.prefix_len = 0;
     a.part_o = reinterpret_cast<float*>(workspace);
     a.part_ml = a.part_o + (size_t)(p.np + p.ns) * T * Hq * D;
     a.out = out;
@@ -955,12 +1025,12 @@ using namespace m355;
 
 extern "C" size_t m355_shared_prefix_attn_workspace_bytes(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len) {
     if (T <= 0 || B <= 0 || max_q <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_ctx <= 0 || prefix_len < 0) return 0;
-    return plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, false).bytes;
+    return plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, 0, false).bytes;
 }
 
 extern "C" size_t m355_paged_attn_decode_scored_workspace_bytes(int B, int Hq, int Hkv, int D, int max_ctx, int prefix_len) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_ctx <= 0 || prefix_len < 0) return 0;
-    return plan_shared_attn(B, B, 1, Hq, Hkv, D, max_ctx, prefix_len, true).bytes;
+    return plan_shared_attn(B, B, 1, Hq, Hkv, D, max_ctx, prefix_len, 0, true).bytes;
 }
 
 extern "C" int m355_shared_prefix_attn(const void* q, const void* kcache, const void* vcache, const int32_t* block_tables,

@@ -209,6 +209,81 @@ def test_gpu_nonfinite_values_reach_only_who_sees_them(dtype, value, m355, cuda)
     check(torch.where(hit, torch.zeros_like(got), got), torch.where(hit, 0.0, want), mag, dtype, score_err(c, q, 0.125))
 
 
+# behind prefixes so long that they are walked once for all, in ranges that are joined
+EXTEND_LONG = [
+    ([20, 33, 1], [20, 33, 1], 3001, 32, 0, False), ([40, 90], [7, 80], 2500, 20, 600, True), ([3, 1], [3, 1], 4100, 16, 0, True),
+    ([40, 600], [2, 3], 1201, 16, 0, False), ([700, 30, 2], [5, 30, 0], 4000, 48, 0, True), ([300, 260], [300, 260], 4101, 16, 0, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout, case", [(x, i) for x in LAYOUTS[:6] for i in range(len(EXTEND_LONG)) if i < 5 or x[0] == 64],
+                         ids=lambda x: f"{x[0]}-{x[1]}-{x[2]}-{str(x[3])[6:]}" if isinstance(x, tuple) else str(x))
+def test_gpu_several_tokens_behind_a_long_prefix(layout, case, m355, cuda):
+    Hq, Hkv, D, dtype = layout
+    own, n, P, block, window, sinks = EXTEND_LONG[case]
+    c = Cache(700 + case, [P + o for o in own], Hkv, D, block, dtype, prefix=P, poison=True, n=n, window=window)
+    T = sum(n)
+    q, sk = _inputs(c, T + 2, Hq, case, sinks)
+    scale = D ** -0.5
+    want, mag, _ = oracle(c, q[:T], n, scale, sk, window)
+    kc, vc, bt, cl = c.device(cuda)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(n)]), dtype=torch.int32, device=cuda)
+    out = torch.full((T + 2, Hq, D), -3.0, dtype=dtype, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=scale, seq_starts=starts, max_q=max(n),
+                                  sinks=None if sk is None else sk.to(cuda), window=window, out=out)
+    check(got[:T], want, mag, dtype, score_err(c, q, scale))
+    assert (out[T:] == -3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_gpu_nonfinite_values_behind_a_long_prefix(dtype, value, m355, cuda):
+    """An infinite or NaN value of a drafted token, and of a prefix token at a window's end, where the prefix is walked once for
+    all: they reach the rows that see them and no other."""
+    P, n = 4096, [4, 4]
+    c = Cache(15, [P + 26, P + 36], 2, 64, 16, dtype, prefix=P)
+    q, _ = _inputs(c, 8, 8, 3, False)
+    for window, (pos, head, column), rows, heads in ((0, (P + 25, 1, 5), [3], slice(4, 8)), (3990, (P + 25 - 3990, 0, 63), [0, 1, 2], slice(0, 4))):
+        want, mag, _ = oracle(c, q, n, 0.125, window=window)
+        page, off = c.slots(0)
+        kept = c.v[page[pos], off[pos], head, column].clone()
+        c.v[page[pos], off[pos], head, column] = value
+        kc, vc, bt, cl = c.device(cuda)
+        c.v[page[pos], off[pos], head, column] = kept
+        st = torch.tensor([0, 4, 8], dtype=torch.int32, device=cuda)
+        got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125, seq_starts=st, max_q=4,
+                                      window=window).cpu()
+        hit = torch.zeros(got.shape, dtype=torch.bool)
+        hit[rows, heads, column] = True
+        assert (~got[hit].isfinite()).all()
+        check(torch.where(hit, torch.zeros_like(got), got), torch.where(hit, 0.0, want), mag, dtype, score_err(c, q, 0.125))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P", [9, 5000])
+@pytest.mark.parametrize("heads", [(8, 2), (64, 2)])
+def test_gpu_more_tokens_than_announced_and_empty_contexts(P, heads, m355, cuda):
+    """Tokens behind max_q of their sequence keep what the output held; a query without a key to see gets zeros, with and
+    without sinks; nothing else changes."""
+    c = Cache(31, [P + 40, P + 3], heads[1], 64, 16, F16, prefix=P, n=[40, 3])
+    q, _ = _inputs(c, 43, heads[0], 1, False)
+    sk = torch.randn((heads[0],), generator=torch.Generator().manual_seed(2)).to(F16)
+    kc, vc, bt, cl = c.device(cuda)
+    st = torch.tensor([0, 40, 43], dtype=torch.int32, device=cuda)
+    full = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=P + 40, scale=0.125, seq_starts=st, max_q=40)
+    out = torch.full_like(full, 5.0)
+    m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=P + 40, scale=0.125, seq_starts=st, max_q=6, out=out)
+    assert (out[6:40] == 5.0).all()
+    want, mag, _ = oracle(c, q, [40, 3], 0.125)
+    for got in (full, torch.cat([out[:6], full[6:40], out[40:]])):
+        check(got, want, mag, F16, score_err(c, q, 0.125))
+    for sinks in (None, sk.to(cuda)):
+        none = m355.shared_prefix_attn(q[:2].to(cuda), kc, vc, bt, torch.zeros_like(cl), prefix_len=P, max_ctx=P + 40, scale=0.125, sinks=sinks)
+        assert (none == 0).all()
+
+
 SCORED = [([1], 0, 16, 0, False), ([1, 2, 33], 0, 16, 0, True), ([31, 300, 65], 7, 16, 0, False), ([700, 5], 64, 20, 0, True),
           ([260, 900], 0, 64, 200, True), ([3, 40], 33, 16, 2, False), ([0, 4], 48, 16, 0, False), ([1500], 1, 128, 0, False)]
 
