@@ -1,15 +1,24 @@
 // Eviction from a paged KV cache by accumulated attention weight: per (sequence, KV head) the last tokens and, of the
 // others, those with the largest scores are kept and copied, in order, to other pages.
 //
-// Two launches.  kv_select: a workgroup per (sequence, KV head) finds the c-th largest score by radix selection (11, 11 and
-// 10 bits of an order-preserving integer image of the score, histograms in LDS; the first digit reaches into the mantissa,
-// so that scores of one magnitude spread over bins), then lists in order the positions above it and the first of those
-// equal to it.  kv_move: a 16-byte piece of a row per lane; reads and writes are whole rows.
+// kv_select: a workgroup per (sequence, KV head) finds the c-th largest score by radix selection (11, 11 and 10 bits of an
+// order-preserving integer image of the score, histograms in LDS; the first digit reaches into the mantissa, so that scores of
+// one magnitude spread over bins), then lists in order the positions above it and the first of those equal to it.  kv_move: a
+// 16-byte piece of a row per lane; reads and writes are whole rows.  A few rows are copied by the selection's workgroup itself.
+// What bounds them: the copy by memory (412 MB in 87 us, 4.7 TB/s, of the 5.2 TB/s of a plain copy); a selection by its chain of
+// barriers and LDS passes, and over long lists by what one CU reads (16 heads of 300 tokens 7 us, 256 of 4096 12 us, 24 of 65536
+// 36 us, of which 10 us for reading and the first histogram, 5 us for the second digit, 3 us for listing the limit's bin, 2 us
+// for the low digits, 9 us for counting and writing; 66 us when the keys were read again for every pass).
 #include "common.h"
 
 namespace m355 {
 
 constexpr int EV_THREADS = 256;
+// Up to so many bytes of K per head (a selection of 256 / of 1024 threads), its workgroup copies the kept rows itself, without
+// a second launch.  Measured, one launch / two, us: 128 rows of 128 bytes of 300 tokens, 16 heads 9.3 / 10.3, of 1000 tokens,
+// 256 heads 13.1 / 14.6; 256 rows 12.0 / 11.3 and 15.8 / 17.0; 512 rows 16.2 / 12.6 and 23.4 / 22.9; of 9000 tokens, 32 heads:
+// 256 rows 15.9 / 18.2, 512 rows 18.8 / 19.0, 1024 rows 24.1 / 19.7.  (And the second launch is 2.5 us of the host's time.)
+constexpr int64_t EV_ONE_LAUNCH = 32768, EV_ONE_LAUNCH_LONG = 65536;
 
 struct EvictArgs {
     unsigned char *kc, *vc;
@@ -84,6 +93,63 @@ __device__ __forceinline__ void each_key(const EvictArgs& a, const Selection& s,
 }
 
 __device__ __forceinline__ bool aligned_scores(const EvictArgs& a) { return (reinterpret_cast<uintptr_t>(a.scores) & 15) == 0; }
+
+// Copies up to `rows` of the m kept rows from entry i0 on; a thread has EV_AHEAD 16-byte pieces of K and of V on their way.
+constexpr int EV_ROWS = 32, EV_AHEAD = 2;
+template <int THREADS>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int hk, int b, int m, int i0, int rows) {
+    const int tid = threadIdx.x;
+    const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hk) * a.keep;
+    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+    const int32_t* dst = a.dst_tables + (int64_t)b * a.max_dst_blocks;
+    const int pieces = a.row_bytes / 16, items = min(rows, m - i0) * pieces;
+    for (int w0 = tid; w0 < items; w0 += THREADS * EV_AHEAD) {
+        int64_t src[EV_AHEAD], put[EV_AHEAD], score_src[EV_AHEAD], score_put[EV_AHEAD];   // (put < 0: dropped)
+        u32x4_t k[EV_AHEAD], v[EV_AHEAD];
+        int from[EV_AHEAD], fb[EV_AHEAD], tb[EV_AHEAD];
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++)   // (clamped: no access leaves the table, whatever became of the scores)
+            from[u] = min(max(kept[i0 + min(w0 + u * THREADS, items - 1) / pieces], 0), a.max_ctx - 1);
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            fb[u] = table[page_of(a, from[u])];
+            tb[u] = dst[page_of(a, a.prefix_len + i0 + min(w0 + u * THREADS, items - 1) / pieces)];
+        }
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            const int w = min(w0 + u * THREADS, items - 1), off = w % pieces * 16, to = a.prefix_len + i0 + w / pieces;
+            const int fo = from[u] - page_of(a, from[u]) * a.block_size, ro = to - page_of(a, to) * a.block_size;
+            const int f = min(max(fb[u], 0), a.num_blocks - 1);
+            src[u] = f * a.block_stride + ((int64_t)fo * a.Hkv + hk) * a.row_bytes + off;
+            k[u] = *reinterpret_cast<const u32x4_t*>(a.kc + src[u]);
+            v[u] = *reinterpret_cast<const u32x4_t*>(a.vc + src[u]);
+            const bool ok = w0 + u * THREADS < items && tb[u] >= 0 && tb[u] < a.num_blocks;
+            put[u] = ok ? tb[u] * a.block_stride + ((int64_t)ro * a.Hkv + hk) * a.row_bytes + off : -1;
+            score_src[u] = ((int64_t)f * a.Hkv + hk) * a.block_size + fo;
+            score_put[u] = ok && off == 0 ? ((int64_t)tb[u] * a.Hkv + hk) * a.block_size + ro : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < EV_AHEAD; u++) {
+            if (put[u] < 0) continue;
+            __builtin_nontemporal_store(k[u], reinterpret_cast<u32x4_t*>(a.kc + put[u]));   // (nobody reads them soon)
+            __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(a.vc + put[u]));
+            if (score_put[u] >= 0) a.scores[score_put[u]] = a.scores[score_src[u]];
+        }
+    }
+    if (i0 == 0 && m > 0) {   // the rest of the last page
+        const int end = a.prefix_len + m, tp = page_of(a, end - 1), tb = dst[tp];
+        if (tb >= 0 && tb < a.num_blocks)
+            for (int i = end - tp * a.block_size + tid; i < a.block_size; i += THREADS)
+                a.scores[((int64_t)tb * a.Hkv + hk) * a.block_size + i] = 0.f;
+    }
+}
+// The selection's own workgroup copies what it has listed.
+template <int THREADS>
+__device__ __forceinline__ void move_listed(const EvictArgs& a, int hk, int b) {
+    __syncthreads();
+    const int n = min(max(a.ctx_lens[b], 0), a.max_ctx) - a.prefix_len, m = min(max(n, 0), a.keep);
+    move_rows<THREADS>(a, hk, b, m, 0, m);
+}
 
 // The bin of the left-th largest of the values counted in hist[0 .. bins); left becomes its rank within that bin.  Called by
 // all threads behind a barrier; ends with one.
@@ -168,9 +234,9 @@ __device__ __forceinline__ void list_kept(const EvictArgs& a, int32_t* kept, int
 
 // Up to THREADS * ITEMS own tokens, their keys in registers (ITEMS = 0: any number, keys are read again for every pass).
 template <int THREADS, int ITEMS>
-__global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
+__device__ __forceinline__ void select_kept(const EvictArgs& a, int hk, int b) {
     __shared__ int hist[2048];
-    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Selection s;
     if (!begin_selection<THREADS>(a, hk, b, s)) return;
@@ -209,6 +275,12 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
     limit = limit << 10 | find_bin<THREADS, 1024>(hist, left);
     list_kept<THREADS>(a, s.kept, s.c, left, [&](auto f) { each([&](int i, uint32_t k, bool in) { f(i, in && k > limit, in && k == limit); }); });
 }
+template <int THREADS, int ITEMS, bool MOVE>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(EvictArgs a) {
+    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv;
+    select_kept<THREADS, ITEMS>(a, hk, b);
+    if (MOVE) move_listed<THREADS>(a, hk, b);
+}
 
 // Exclusive prefix sum over the wave, and its total.
 template <int CTRL, int ROW_MASK = 0xf>
@@ -230,12 +302,12 @@ __device__ __forceinline__ int wave_scan(int v, int& total) {
 // again.  Where equal scores make them too many for the lists, they are read again each time.
 constexpr int EV_LONG = 65536, EV_LIST = 256;
 template <int N>
-__global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
+__device__ __forceinline__ void select_kept_long(const EvictArgs& a, int hk, int b) {
     constexpr int THREADS = 1024, WAVES = THREADS / 64;
     __shared__ __attribute__((aligned(16))) uint16_t upper[N];
     __shared__ uint16_t list_at[WAVES][EV_LIST], list_low[WAVES][EV_LIST];
     __shared__ int hist[2048], too_many, wave_gt[WAVES], wave_eq[WAVES];
-    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Selection s;
     if (!begin_selection<THREADS>(a, hk, b, s)) return;
@@ -407,55 +479,17 @@ __global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
         at += total;
     });
 }
+template <int N, bool MOVE>
+__global__ __launch_bounds__(1024) void kv_select_long_kernel(EvictArgs a) {
+    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv;
+    select_kept_long<N>(a, hk, b);
+    if (MOVE) move_listed<1024>(a, hk, b);
+}
 
-// A workgroup per (sequence, KV head, EV_ROWS kept tokens); a lane has EV_AHEAD 16-byte pieces of K and of V on their way.
-constexpr int EV_ROWS = 32, EV_AHEAD = 2;
+// A workgroup per (sequence, KV head, EV_ROWS kept tokens).
 __global__ __launch_bounds__(EV_THREADS) void kv_move_kernel(EvictArgs a, int chunks) {
-    const int hk = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv % chunks, b = blockIdx.x / a.Hkv / chunks, tid = threadIdx.x;
-    const int m = a.new_lens[b] - a.prefix_len;
-    const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hk) * a.keep;
-    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    const int32_t* dst = a.dst_tables + (int64_t)b * a.max_dst_blocks;
-    const int pieces = a.row_bytes / 16, i0 = chunk * EV_ROWS, items = min(EV_ROWS, m - i0) * pieces;
-    for (int w0 = tid; w0 < items; w0 += EV_THREADS * EV_AHEAD) {
-        int64_t src[EV_AHEAD], put[EV_AHEAD], score_src[EV_AHEAD], score_put[EV_AHEAD];   // (put < 0: dropped)
-        u32x4_t k[EV_AHEAD], v[EV_AHEAD];
-        int from[EV_AHEAD], fb[EV_AHEAD], tb[EV_AHEAD];
-#pragma unroll
-        for (int u = 0; u < EV_AHEAD; u++)   // (clamped: no access leaves the table, whatever became of the scores)
-            from[u] = min(max(kept[i0 + min(w0 + u * EV_THREADS, items - 1) / pieces], 0), a.max_ctx - 1);
-#pragma unroll
-        for (int u = 0; u < EV_AHEAD; u++) {
-            fb[u] = table[page_of(a, from[u])];
-            tb[u] = dst[page_of(a, a.prefix_len + i0 + min(w0 + u * EV_THREADS, items - 1) / pieces)];
-        }
-#pragma unroll
-        for (int u = 0; u < EV_AHEAD; u++) {
-            const int w = min(w0 + u * EV_THREADS, items - 1), off = w % pieces * 16, to = a.prefix_len + i0 + w / pieces;
-            const int fo = from[u] - page_of(a, from[u]) * a.block_size, ro = to - page_of(a, to) * a.block_size;
-            const int f = min(max(fb[u], 0), a.num_blocks - 1);
-            src[u] = f * a.block_stride + ((int64_t)fo * a.Hkv + hk) * a.row_bytes + off;
-            k[u] = *reinterpret_cast<const u32x4_t*>(a.kc + src[u]);
-            v[u] = *reinterpret_cast<const u32x4_t*>(a.vc + src[u]);
-            const bool ok = w0 + u * EV_THREADS < items && tb[u] >= 0 && tb[u] < a.num_blocks;
-            put[u] = ok ? tb[u] * a.block_stride + ((int64_t)ro * a.Hkv + hk) * a.row_bytes + off : -1;
-            score_src[u] = ((int64_t)f * a.Hkv + hk) * a.block_size + fo;
-            score_put[u] = ok && off == 0 ? ((int64_t)tb[u] * a.Hkv + hk) * a.block_size + ro : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < EV_AHEAD; u++) {
-            if (put[u] < 0) continue;
-            __builtin_nontemporal_store(k[u], reinterpret_cast<u32x4_t*>(a.kc + put[u]));   // (nobody reads them soon)
-            __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(a.vc + put[u]));
-            if (score_put[u] >= 0) a.scores[score_put[u]] = a.scores[score_src[u]];
-        }
-    }
-    if (chunk == 0 && m > 0) {   // the rest of the last page
-        const int end = a.prefix_len + m, tp = page_of(a, end - 1), tb = dst[tp];
-        if (tb >= 0 && tb < a.num_blocks)
-            for (int i = end - tp * a.block_size + tid; i < a.block_size; i += EV_THREADS)
-                a.scores[((int64_t)tb * a.Hkv + hk) * a.block_size + i] = 0.f;
-    }
+    const int hk = blockIdx.x % a.Hkv, chunk = blockIdx.x / a.Hkv % chunks, b = blockIdx.x / a.Hkv / chunks;
+    move_rows<EV_THREADS>(a, hk, b, a.new_lens[b] - a.prefix_len, chunk * EV_ROWS, EV_ROWS);
 }
 
 }  // namespace m355
@@ -494,12 +528,18 @@ extern "C" int m355_kv_evict(void* kcache, void* vcache, float* scores, const in
                 block_size, max_blocks, max_dst_blocks, block_stride_bytes, page_mul, page_shift, max_ctx, prefix_len, keep, recent, kept, new_lens};
     hipStream_t st = (hipStream_t)stream;
     const int64_t own = max_ctx - (int64_t)prefix_len;
-    if (own <= 1024) kv_select_kernel<256, 4><<<B * Hkv, 256, 0, st>>>(a);
-    else if (own <= 16384) kv_select_long_kernel<16384><<<B * Hkv, 1024, 0, st>>>(a);
-    else if (own <= EV_LONG) kv_select_long_kernel<EV_LONG><<<B * Hkv, 1024, 0, st>>>(a);
-    else kv_select_kernel<1024, 0><<<B * Hkv, 1024, 0, st>>>(a);
+    const bool move = most * row_bytes <= (own <= 1024 ? EV_ONE_LAUNCH : EV_ONE_LAUNCH_LONG);
+    const int wgs = B * Hkv;
+#define M355_EV(KERNEL, THREADS, ...)                                  \
+    if (move) KERNEL<__VA_ARGS__, true><<<wgs, THREADS, 0, st>>>(a);   \
+    else KERNEL<__VA_ARGS__, false><<<wgs, THREADS, 0, st>>>(a)
+    if (own <= 1024) { M355_EV(kv_select_kernel, 256, 256, 4); }
+    else if (own <= 16384) { M355_EV(kv_select_long_kernel, 1024, 16384); }
+    else if (own <= EV_LONG) { M355_EV(kv_select_long_kernel, 1024, EV_LONG); }
+    else { M355_EV(kv_select_kernel, 1024, 1024, 0); }
+#undef M355_EV
     M355_LAUNCH_CHECK("kv_select_kernel");
-    if (chunks) {
+    if (chunks && !move) {
         kv_move_kernel<<<(int)(B * Hkv * chunks), EV_THREADS, 0, st>>>(a, (int)chunks);
         M355_LAUNCH_CHECK("kv_move_kernel");
     }

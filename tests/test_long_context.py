@@ -323,7 +323,8 @@ def test_gpu_scored_decode(layout, case, m355, cuda):
 EVICT = [([1], 0, 16, 4, 1), ([5, 6, 7], 0, 16, 6, 2), ([100, 300, 129], 32, 16, 64, 10), ([1000, 17], 0, 20, 33, 33),
          ([700, 300], 64, 64, 256, 0), ([4, 2], 16, 16, 1, 0), ([3000, 64], 0, 128, 1025, 100), ([0, 9], 48, 16, 8, 3),
          ([1024, 1025], 0, 16, 500, 1), ([17000, 16384], 64, 64, 3333, 128), ([66000, 1], 0, 128, 4097, 5),
-         ([3000, 2001], 40, 20, 700, 7), ([40001, 19000], 0, 64, 10000, 77)]
+         ([3000, 2001], 40, 20, 700, 7), ([40001, 19000], 0, 64, 10000, 77),
+         ([30000, 17], 0, 64, 100, 9), ([70000, 5], 0, 128, 60, 3), ([900, 1000], 32, 16, 520, 40)]
 
 
 def evict_oracle(c, keep, recent):
