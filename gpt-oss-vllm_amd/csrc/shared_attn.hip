@@ -14,6 +14,13 @@
 //                            holds one row's scores of 16 keys (lane ^ 32 the other 16).
 //   O^T[d][row] += V^T P^T   the probabilities, rounded to the cache's type where they sit (the matrix core takes 16-bit
 //                            operands; o and l stay fp32), are the B operand; V^T comes from LDS through the transposing read.
+//
+// What bounds it.  Own tokens: memory (32 sequences of 2500 tokens, 8 KV heads of 64: 164 MB in 35 us, 4.7 TB/s; a plain copy
+// of the card: 5.2).  A walk over a prefix: the chain of one wave per SIMD, products, exponentials and LDS reads behind one
+// another (1.0 us per 64 keys of 128 rows, D 64, where the matrix cores need 0.25), so that two workgroups per CU get 1.6 times
+// as much done; many rows: exponentials beside the products (6 prompts of 150 to 420 tokens behind 8192, 226 GFLOP: 322 us, 0.70
+// PFLOP/s of the 1.2 that a large product reaches).  Tried without gain: 64 keys at a time, a K tile's fragments read a tile
+// ahead, four or five tiles in LDS instead of three.  Few tokens: launches (7 us for one, 10 for the ranges and their joining).
 #include "common.h"
 
 #include <cmath>
@@ -772,7 +779,9 @@ __device__ __forceinline__ void merge_part(const SharedAttnArgs& a, int id) {
 }
 
 // Adds the own tokens' weights, summed over the group's query heads: a workgroup per (sequence, KV head, SA_SCORE_KEYS
-// tokens), which joins the heads' (m, l) once more for itself instead of waiting for another launch.
+// tokens), which joins the heads' (m, l) once more for itself instead of waiting for another launch.  The logits that the walk
+// leaves behind and this reads are 4 bytes per key and query head beside 4 D per key and KV head of K and V: 20 of 205 MB twice
+// for 32 sequences of 2500 tokens, D 64, where the walk takes 47 us with them, 35 without, and this launch 10.
 constexpr int SA_SCORE_KEYS = 4 * SA_THREADS;
 template <typename E>
 __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int pieces) {
@@ -903,6 +912,9 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     SharedAttnPlan p;
     max_q = max_q < T ? max_q : T;
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
+    // Rows per workgroup.  32: the four waves share the keys (4 tokens of 8 heads on 8192 keys 13.4 us, with 128 rows 15.8); 128:
+    // they share the tiles; 256 (D 64, many rows): every fragment read from LDS serves two row sets (512 tokens of 64 heads on
+    // 8192 keys 120 us, with 128 rows 134; 600 tokens 144 and 147, 1700 tokens 331 and 341).
     p.prefix_rows = R <= 32 ? 32 : D == 64 && R * Hkv >= 32768 && !scored ? 256 : 128;
     p.own_rows = max_q * G > 32 && !scored ? 128 : 32;
     const double merge = (double)T * Hq * D * 4 / 2500;

@@ -376,8 +376,8 @@ M355_API int m355_norm_qkv_rope_kv_write(const void* x_f16, const void* delta_f1
  *   first tokens of the sequences, max_q (host) the longest one's number of tokens; NULL: one token per sequence (T == B).
  *   A sequence's n new tokens are the last n of its ctx_lens positions and see the keys up to their own (window > 0: the
  *   last `window` of them).  The first prefix_len positions (host; 0: none) are the same tokens for every sequence: they are
- *   read through row 0 of block_tables, once for all, the others through the sequence's own row.  prefix_len need not end a
- *   page.  Queries may lie anywhere (a prefix_len beyond a sequence's end only hides what it does not see).  Rows that see
+ *   read through row 0 of block_tables (once for all, where that is cheaper than again for every sequence), the others through
+ *   the sequence's own row.  prefix_len need not end a page.  Queries may lie anywhere (a prefix_len beyond a sequence's end only hides what it does not see).  Rows that see
  *   nothing become 0; rows of q behind seq_starts[B], and a sequence's tokens behind max_q, leave `out` as it was.
  *   Infinities and NaN in K or V reach the queries that see them and no others.
  *   With one sequence per row and prefix_len = 0 it is m355_paged_attn_decode_ex.
