@@ -259,6 +259,37 @@ __device__ __forceinline__ void put_out(const SharedAttnArgs& a, int token, int 
     for (int i = 0; i < 4; i++) out[i] = (E)(num[i] * inv);
 }
 
+// Adds the weights of a sequence's own tokens that its only range has left logits of (from position 0 on); fin: every head's
+// maximum and inverse denominator.
+__device__ __forceinline__ void add_weights(const SharedAttnArgs& a, int b, int hk, const float (*fin)[2]) {
+    const int ctx = min(a.ctx_lens[b], a.max_ctx), lo = max(window_lo(a, ctx - 1), a.folded);
+    const float* x = a.logits + ((int64_t)b * a.Hq + hk * a.G) * a.lstride;
+    for (int rel = lo / 4 * 4 + 4 * (int)threadIdx.x; rel < ctx; rel += 4 * SA_THREADS) {
+        float* slot[4];
+        float old[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int key = rel + u;
+            slot[u] = nullptr;
+            if (key >= ctx || key < lo) continue;
+            const int page = page_of(a, key), blk = a.tables[(int64_t)b * a.max_blocks + page];
+            if (blk < 0 || blk >= a.num_blocks) continue;   // no score is written outside the cache
+            slot[u] = a.scores + ((int64_t)blk * a.Hkv + hk) * a.block_size + (key - page * a.block_size);
+            old[u] = *slot[u];
+        }
+        float4_t w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int g = 0; g < a.G; g++) {
+            const float4_t v = *reinterpret_cast<const float4_t*>(x + (int64_t)g * a.lstride + rel);
+#pragma unroll
+            for (int u = 0; u < 4; u++) w[u] += __builtin_amdgcn_exp2f(v[u] - fin[g][0]) * fin[g][1];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (slot[u]) *slot[u] = old[u] + w[u];
+    }
+}
+
 // Shape of a workgroup's walk.  RW = 4: every wave holds 32 * QT rows, tiles of 64 keys are shared, NS of them in LDS or on
 // their way.  RW = 1: one set of 32 rows, the waves take tiles of 32 keys in turn, each in LDS of its own; a tile is read
 // into registers whole, and the next one requested into its place before the softmax.
@@ -617,6 +648,24 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         }
         __syncthreads();
         const int nrows = min(32, row_end - row0);
+        if constexpr (SCORED) {
+            if (direct) {   // (the rows are one token's, all of the KV head's)
+                __shared__ float fin[32][2];
+                if (tid < nrows) {
+                    float m = wm[0][tid], l = 0.f, m_all, den, back;
+#pragma unroll
+                    for (int w = 1; w < SA_WAVES; w++) m = fmaxf(m, wm[w][tid]);
+#pragma unroll
+                    for (int w = 0; w < SA_WAVES; w++) l += (wm[w][tid] == m ? 1.0f : __builtin_amdgcn_exp2f(wm[w][tid] - m)) * wl[w][tid];
+                    start_with_sink<E>(a, hk * a.G + tid, m_all, den);
+                    join_stats<1>(RangeStat{true, m, l}, m_all, den, back);
+                    fin[tid][0] = m_all;
+                    fin[tid][1] = inverse(den);
+                }
+                __syncthreads();   // (and the waves' logits)
+                add_weights(a, own_b, hk, fin);
+            }
+        }
         for (int i = tid; i < nrows * CH; i += SA_THREADS) {
             const int r32 = i / CH, c = i % CH;
             float m = wm[0][r32];
@@ -695,7 +744,7 @@ __device__ __forceinline__ void own_part(const SharedAttnArgs& a, unsigned char*
     const int hk = id % a.Hkv, unit = id / a.Hkv, split = unit % a.ns;
     const int b = unit / a.ns / row_sets, set = unit / a.ns % row_sets;
     const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    const int k0 = a.prefix_len + split * a.so, folded = SCORED ? 0 : a.folded;
+    const int k0 = a.prefix_len + split * a.so, folded = a.folded;
     const int pages_from = page_of(a, k0) + (k0 >= folded ? split_page(a, folded) : 0);
     fetch_pages<D, RW>(a, smem, table, pages_from, folded);
     const SeqSpan s = seq_span(a, b);
@@ -707,7 +756,7 @@ __device__ __forceinline__ void own_part(const SharedAttnArgs& a, unsigned char*
     const int pos[1] = {pos0 + row / a.G}, lo[1] = {window_lo(a, pos[0])};
     const int kbeg = max(k0, window_lo(a, pos0 + row0 / a.G));
     int kend = min(k0 + a.so, pos0 + (row_end - 1) / a.G + 1);
-    const bool direct = !SCORED && a.direct;
+    const bool direct = a.direct;
     if (kbeg >= kend && !direct) return;
     kend = max(kend, kbeg);   // (direct: rows that see nothing are written all the same)
     // (scored: the logits are addressed from the range's start in steps of a tile, so the walk starts on one)
@@ -931,7 +980,7 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     double t = cut_keys(P, prefix_units, cost(false, p.prefix_rows, p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0), p.np, p.sp);
     t += cut_keys(own, own_units, cost(true, p.own_rows, 0), p.ns, p.so) - (P && own > 0 ? 7000 : 0);
     // One range per sequence, which takes the prefix along, instead: every sequence reads the prefix again (from the L2s), but
-    // no outputs are left to be joined, nor is there a second launch (2500 ns of the host's time, and a base of 5500 for 7000).
+    // no outputs are left to be joined, nor is there a second launch (about 3000 ns of the host's time, and a base of 5500 for 7000).
     // Fitted to 31 pairs, among them (us of kernels, ranges and joining / one range): 4 sequences of 200 + 33 tokens 9.6 / 7.2,
     // 16 of 500 + 100 13.1 / 9.5, 32 of 1500 + 60 14.7 / 15.7, 32 of 8192 + 512 22.9 / 58.9; 45 prompts of 42 to 81 tokens
     // behind 9 92 / 38, 24 of 200 to 300 behind 512 282 / 173, 6 of 150 to 420 behind 8192 364 / 410.
@@ -944,16 +993,17 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
         w.uneven = 0;
         return cut_cost(keys, own_units, w, (keys + 127) / 128 * 128) + uneven / (c < 1 ? 1 : c) - (p.own_rows == 32 ? 1500 : 0);
     };
-    p.direct = !scored && one_range(P, own) < t + 2500;
+    // (scored: one row set; 32 of 200 + 100 to 300 tokens 17.2 / 13.5, 64 of 500 to 1000 44.1 / 37.8, 9 of 2278 + 20 19.5 / 32.6)
+    p.direct = (!scored || G <= 32) && one_range(P, own) < t + 3000;
     if (p.direct) p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
-    p.lstride = (int)((own + 127) / 128 * 128);
+    p.lstride = (int)(((p.direct ? max_ctx : own) + 127) / 128 * 128);
     p.logit_floats = scored ? rows * (size_t)p.lstride : 0;
     p.bytes = (p.part_floats + p.logit_floats) * sizeof(float);
     if (window > 0 && !scored && !p.direct) {   // (a row set sees its queries' positions and the window in front of the first)
         const int64_t seen = (int64_t)window + (p.own_rows == 32 ? max_q : 128 / G + 1);
-        if (seen < max_ctx && one_range(0, seen) < t + 2500) p.direct = true, p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
+        if (seen < max_ctx && one_range(0, seen) < t + 3000) p.direct = true, p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
     }
     p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_SCORE_KEYS + 1);
     return p;

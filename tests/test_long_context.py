@@ -285,7 +285,8 @@ def test_gpu_more_tokens_than_announced_and_empty_contexts(P, heads, m355, cuda)
 
 
 SCORED = [([1], 0, 16, 0, False), ([1, 2, 33], 0, 16, 0, True), ([31, 300, 65], 7, 16, 0, False), ([700, 5], 64, 20, 0, True),
-          ([260, 900], 0, 64, 200, True), ([3, 40], 33, 16, 2, False), ([0, 4], 48, 16, 0, False), ([1500], 1, 128, 0, False)]
+          ([260, 900], 0, 64, 200, True), ([3, 40], 33, 16, 2, False), ([0, 4], 48, 16, 0, False), ([1500], 1, 128, 0, False),
+          ([2000, 3], 3000, 16, 0, True), ([33, 2100], 15, 16, 700, False), ([200, 150, 7], 50, 20, 90, True)]
 
 
 @pytest.mark.gpu
