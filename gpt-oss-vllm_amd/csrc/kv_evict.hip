@@ -6,19 +6,21 @@
 // one magnitude spread over bins), then lists in order the positions above it and the first of those equal to it.  kv_move: a
 // 16-byte piece of a row per lane; reads and writes are whole rows.  A few rows are copied by the selection's workgroup itself.
 // What bounds them: the copy by memory (412 MB in 87 us, 4.7 TB/s, of the 5.2 TB/s of a plain copy); a selection by its chain of
-// barriers and LDS passes, and over long lists by what one CU reads (16 heads of 300 tokens 7 us, 256 of 4096 12 us, 24 of 65536
+// barriers and LDS passes, and over long lists by what one CU reads (16 heads of 300 tokens 7 us, 256 of 4096 11 us, 24 of 65536
 // 36 us, of which 10 us for reading and the first histogram, 5 us for the second digit, 3 us for listing the limit's bin, 2 us
 // for the low digits, 9 us for counting and writing; 66 us when the keys were read again for every pass).
 #include "common.h"
 
+#include <type_traits>
+
 namespace m355 {
 
 constexpr int EV_THREADS = 256;
-// Up to so many bytes of K per head (a selection of 256 / of 1024 threads), its workgroup copies the kept rows itself, without
-// a second launch.  Measured, one launch / two, us: 128 rows of 128 bytes of 300 tokens, 16 heads 9.3 / 10.3, of 1000 tokens,
-// 256 heads 13.1 / 14.6; 256 rows 12.0 / 11.3 and 15.8 / 17.0; 512 rows 16.2 / 12.6 and 23.4 / 22.9; of 9000 tokens, 32 heads:
-// 256 rows 15.9 / 18.2, 512 rows 18.8 / 19.0, 1024 rows 24.1 / 19.7.  (And the second launch is 2.5 us of the host's time.)
-constexpr int64_t EV_ONE_LAUNCH = 32768, EV_ONE_LAUNCH_LONG = 65536;
+// Up to so many bytes of K per head, the selection's workgroup copies the kept rows itself, without a second launch.  Measured,
+// one launch / two, us: rows of 128 bytes, 128 of 300 tokens, 16 heads 8.4 / 10.1; of 1000 tokens, 256 heads, 128 rows 11.7 /
+// 13.4, 512 rows 20.2 / 21.7; 16 heads, 512 rows 12.3 / 10.8; of 9000 tokens, 32 heads, 512 rows 18.8 / 19.0, 1024 rows 24.1 /
+// 19.7.  (And the second launch is 2.5 us of the host's time.)
+constexpr int64_t EV_ONE_LAUNCH = 65536;
 
 struct EvictArgs {
     unsigned char *kc, *vc;
@@ -315,26 +317,37 @@ __device__ __forceinline__ void select_kept_long(const EvictArgs& a, int hk, int
     if (tid == 0) too_many = 0;
     clear_bins<THREADS>(hist, 2048);
     {
-        // pages of a multiple of 8 tokens: a lane's eight scores lie side by side (own tokens start on a page)
-        const bool vec = a.block_size % 8 == 0 && aligned_scores(a);
+        // pages of a multiple of 8 (4) tokens: a lane's eight (twice four) scores lie side by side (own tokens start on a page)
+        const int side = !aligned_scores(a) ? 1 : a.block_size % 8 == 0 ? 8 : a.block_size % 4 == 0 ? 4 : 1;
         for (int q0 = 0; q0 < blocks; q0 += 4) {
             float sc[4][8];
-            if (vec) {
-                int off[4], blk[4];
+            auto load = [&](auto parts_c) {   // parts of 8 / parts tokens
+                constexpr int PARTS = decltype(parts_c)::value, W = 8 / PARTS;
+                int off[4][PARTS], blk[4][PARTS];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int i = min(run + (q0 + q) * 512 + lane * 8, (s.cand - 1) & ~7), pos = a.prefix_len + i, page = page_of(a, pos);
-                    off[q] = pos - page * a.block_size;
-                    blk[q] = s.table[page];
-                }
+                for (int q = 0; q < 4; q++)
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const float4_t* from = reinterpret_cast<const float4_t*>(
-                        a.scores + ((int64_t)min(max(blk[q], 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + off[q]);
-                    const float4_t x = from[0], y = from[1];
+                    for (int h = 0; h < PARTS; h++) {
+                        const int i = min(run + (q0 + q) * 512 + lane * 8 + h * W, (s.cand - 1) & ~(W - 1)), pos = a.prefix_len + i;
+                        const int page = page_of(a, pos);
+                        off[q][h] = pos - page * a.block_size;
+                        blk[q][h] = s.table[page];
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[q][e] = x[e], sc[q][4 + e] = y[e];
-                }
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const int h = e / W;
+                        const float4_t x = *reinterpret_cast<const float4_t*>(
+                            a.scores + ((int64_t)min(max(blk[q][h], 0), a.num_blocks - 1) * a.Hkv + hk) * a.block_size + off[q][h] + e % W);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) sc[q][e + c] = x[c];
+                    }
+            };
+            if (side == 8) {
+                load(std::integral_constant<int, 1>{});
+            } else if (side == 4) {
+                load(std::integral_constant<int, 2>{});
             } else {
 #pragma unroll
                 for (int q = 0; q < 4; q++)
@@ -528,12 +541,16 @@ extern "C" int m355_kv_evict(void* kcache, void* vcache, float* scores, const in
                 block_size, max_blocks, max_dst_blocks, block_stride_bytes, page_mul, page_shift, max_ctx, prefix_len, keep, recent, kept, new_lens};
     hipStream_t st = (hipStream_t)stream;
     const int64_t own = max_ctx - (int64_t)prefix_len;
-    const bool move = most * row_bytes <= (own <= 1024 ? EV_ONE_LAUNCH : EV_ONE_LAUNCH_LONG);
+    const bool move = most * row_bytes <= EV_ONE_LAUNCH;
     const int wgs = B * Hkv;
 #define M355_EV(KERNEL, THREADS, ...)                                  \
     if (move) KERNEL<__VA_ARGS__, true><<<wgs, THREADS, 0, st>>>(a);   \
     else KERNEL<__VA_ARGS__, false><<<wgs, THREADS, 0, st>>>(a)
-    if (own <= 1024) { M355_EV(kv_select_kernel, 256, 256, 4); }
+    // Keys in registers, eight to each of 512 threads, several workgroups per CU; four to each of 1024 if two of those per CU hold
+    // all heads (256 heads of up to 4096 tokens 10.6 us, with 512 threads 13.3; 664 of 1000 26.6 and 16.5; 632 of 3300 29.8 and
+    // 18.4).  In LDS beyond: 12.3, 33 and 36.5 us on these.
+    if (own <= 4096 && own > 1024 && wgs <= 512) { M355_EV(kv_select_kernel, 1024, 1024, 4); }
+    else if (own <= 4096) { M355_EV(kv_select_kernel, 512, 512, 8); }
     else if (own <= 16384) { M355_EV(kv_select_long_kernel, 1024, 16384); }
     else if (own <= EV_LONG) { M355_EV(kv_select_long_kernel, 1024, EV_LONG); }
     else { M355_EV(kv_select_kernel, 1024, 1024, 0); }

@@ -325,7 +325,9 @@ EVICT = [([1], 0, 16, 4, 1), ([5, 6, 7], 0, 16, 6, 2), ([100, 300, 129], 32, 16,
          ([700, 300], 64, 64, 256, 0), ([4, 2], 16, 16, 1, 0), ([3000, 64], 0, 128, 1025, 100), ([0, 9], 48, 16, 8, 3),
          ([1024, 1025], 0, 16, 500, 1), ([17000, 16384], 64, 64, 3333, 128), ([66000, 1], 0, 128, 4097, 5),
          ([3000, 2001], 40, 20, 700, 7), ([40001, 19000], 0, 64, 10000, 77),
-         ([30000, 17], 0, 64, 100, 9), ([70000, 5], 0, 128, 60, 3), ([900, 1000], 32, 16, 520, 40)]
+         ([30000, 17], 0, 64, 100, 9), ([70000, 5], 0, 128, 60, 3), ([900, 1000], 32, 16, 520, 40),
+         ([4096, 4097, 513], 16, 16, 1500, 64), ([4096, 2050, 1025], 0, 64, 100, 100), ([1100] * 172, 0, 20, 40, 4), ([4000, 600] * 87, 0, 64, 700, 9),
+         ([6000, 17001], 40, 20, 700, 7), ([5003, 30], 30, 10, 300, 5), ([7007, 4098], 24, 12, 6001, 1)]
 
 
 def evict_oracle(c, keep, recent):
