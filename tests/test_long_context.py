@@ -608,6 +608,66 @@ def test_gpu_capture_and_replay(m355, cuda):
 
 
 @pytest.mark.gpu
+def test_gpu_two_streams_and_two_graphs_of_joined_ranges(m355, cuda):
+    """Long prefixes and long lists (ranges that are joined, rows that a second launch copies), on two streams at once and as
+    two captured graphs replayed at once, each with a workspace of its own: the results of calls one after the other."""
+    P, keep, own = 4096, 700, (2000, 900, 7)
+    sides = []
+    for seed in (1, 2):
+        c = Cache(80 + seed, [P + o for o in own], 4, 64, 16, F16, prefix=P, dst=P + keep)
+        kc, vc, bt, cl = c.device(cuda)
+        q = (1.5 * torch.randn((3, 32, 64), generator=torch.Generator().manual_seed(seed))).to(F16).to(cuda)
+        need = max(m355.shared_prefix_attn_workspace_bytes(3, 3, 1, 32, 4, 64, P + 2000, P), m355.paged_attn_decode_scored_workspace_bytes(3, 32, 4, 64, P + 2000, P))
+        sides.append(dict(first=[kc, vc, c.scores.to(cuda)], caches=[kc.clone(), vc.clone(), c.scores.to(cuda)], bt=bt, cl=cl, dst=c.dst.to(cuda),
+                          q=q, ws=torch.empty(need, dtype=torch.uint8, device=cuda), outs=[torch.empty_like(q) for _ in range(2)],
+                          kept=torch.empty((3, 4, keep), dtype=torch.int32, device=cuda), lens=torch.empty(3, dtype=torch.int32, device=cuda),
+                          stream=torch.cuda.Stream(device=cuda)))
+
+    def run(s):
+        k, v, sc = s["caches"]
+        m355.shared_prefix_attn(s["q"], k, v, s["bt"], s["cl"], prefix_len=P, max_ctx=P + 2000, scale=0.125, workspace=s["ws"], out=s["outs"][0])
+        m355.paged_attn_decode_scored(s["q"], k, v, sc, s["bt"], s["cl"], prefix_len=P, max_ctx=P + 2000, scale=0.125, workspace=s["ws"], out=s["outs"][1])
+        m355.kv_evict(k, v, sc, s["bt"], s["cl"], s["dst"], keep=keep, recent=9, prefix_len=P, max_ctx=P + 2000, kept=s["kept"], new_lens=s["lens"])
+
+    def reset(s):
+        for t, f in zip(s["caches"], s["first"]):
+            t.copy_(f)
+        for t in s["outs"] + [s["kept"], s["lens"]]:
+            t.zero_()
+        s["ws"].fill_(255)
+
+    def results(s):
+        return [t.clone() for t in s["outs"] + s["caches"] + [s["kept"], s["lens"]]]
+
+    want = []
+    for s in sides:
+        reset(s)
+        run(s)
+        torch.cuda.synchronize()
+        want.append(results(s))
+    graphs = []
+    for s in sides:
+        s["stream"].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s["stream"]):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s["stream"]):
+                run(s)
+            graphs.append(g)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for s in sides:
+            reset(s)
+        torch.cuda.synchronize()
+        for s, g in zip(sides, graphs):
+            with torch.cuda.stream(s["stream"]):
+                run(s) if turn % 2 else g.replay()
+        torch.cuda.synchronize()
+        for s, w in zip(sides, want):
+            for got, exp in zip(results(s), w):
+                assert torch.equal(got, exp)
+
+
+@pytest.mark.gpu
 def test_gpu_equals_the_paged_decode_kernel(m355, cuda):
     """Without a prefix the new entry point computes what m355_paged_attn_decode_ex computes, and a batch whose rows name the
     shared pages gives the same with and without prefix_len."""
