@@ -983,7 +983,7 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     // no outputs are left to be joined, nor is there a second launch (about 3000 ns of the host's time, and a base of 5500 for 7000).
     // Fitted to 31 pairs, among them (us of kernels, ranges and joining / one range): 4 sequences of 200 + 33 tokens 9.6 / 7.2,
     // 16 of 500 + 100 13.1 / 9.5, 32 of 1500 + 60 14.7 / 15.7, 32 of 8192 + 512 22.9 / 58.9; 45 prompts of 42 to 81 tokens
-    // behind 9 92 / 38, 24 of 200 to 300 behind 512 282 / 173, 6 of 150 to 420 behind 8192 364 / 410.
+    // behind 9 92 / 35, 24 of 200 to 300 behind 512 282 / 160, 6 of 150 to 420 behind 8192 364 / 410.
     auto one_range = [&](int64_t keys_prefix, int64_t keys_own) {
         CutCost w = cost(true, p.own_rows, 0);
         const int64_t keys = keys_prefix + keys_own;
@@ -994,8 +994,13 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
         return cut_cost(keys, own_units, w, (keys + 127) / 128 * 128) + uneven / (c < 1 ? 1 : c) - (p.own_rows == 32 ? 1500 : 0);
     };
     // (scored: one row set; 32 of 200 + 100 to 300 tokens 17.2 / 13.5, 64 of 500 to 1000 44.1 / 37.8, 9 of 2278 + 20 19.5 / 32.6)
-    p.direct = (!scored || G <= 32) && one_range(P, own) < t + 3000;
-    if (p.direct) p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
+    auto take_one_range = [&] {
+        p.direct = true;
+        p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
+        p.prefix_rows = p.own_rows;   // (no kernel with more LDS and registers than the own walks use)
+    };
+    p.direct = false;
+    if ((!scored || G <= 32) && one_range(P, own) < t + 3000) take_one_range();
     const size_t rows = (size_t)T * Hq;
     p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
     p.lstride = (int)(((p.direct ? max_ctx : own) + 127) / 128 * 128);
@@ -1003,7 +1008,7 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
     p.bytes = (p.part_floats + p.logit_floats) * sizeof(float);
     if (window > 0 && !scored && !p.direct) {   // (a row set sees its queries' positions and the window in front of the first)
         const int64_t seen = (int64_t)window + (p.own_rows == 32 ? max_q : 128 / G + 1);
-        if (seen < max_ctx && one_range(0, seen) < t + 3000) p.direct = true, p.np = 0, p.ns = 1, p.so = (int)((max_ctx + 127) / 128 * 128);
+        if (seen < max_ctx && one_range(0, seen) < t + 3000) take_one_range();
     }
     p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_SCORE_KEYS + 1);
     return p;
