@@ -238,6 +238,18 @@ def test_gpu_several_tokens_behind_a_long_prefix(layout, case, m355, cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gpu_many_sequences_on_a_long_prefix(dtype, m355, cuda):
+    own = [1 + b % 5 for b in range(515)]
+    c = Cache(41, [1500 + o for o in own], 8, 64, 16, dtype, prefix=1500, poison=True)
+    q, sk = _inputs(c, len(own), 64, 9, True)
+    want, mag, _ = oracle(c, q, [1] * len(own), 0.125, sk)
+    kc, vc, bt, cl = c.device(cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=1500, max_ctx=max(c.ctx), scale=0.125, sinks=sk.to(cuda))
+    check(got, want, mag, dtype, score_err(c, q, 0.125))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
 def test_gpu_nonfinite_values_behind_a_long_prefix(dtype, value, m355, cuda):
     """An infinite or NaN value of a drafted token, and of a prefix token at a window's end, where the prefix is walked once for
