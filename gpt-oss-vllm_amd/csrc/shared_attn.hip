@@ -67,12 +67,13 @@ __device__ __forceinline__ int page_of(const SharedAttnArgs& a, int key) {
     return (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
 }
 // What a sequence's row range and positions are.  Everything is clamped to what the arguments allow.
+__device__ __forceinline__ int context_of(const SharedAttnArgs& a, int b) { return min(max(a.ctx_lens[b], 0), a.max_ctx); }
 struct SeqSpan {
     int t0, n, ctx;   // first token, number of tokens, cached tokens
 };
 __device__ __forceinline__ SeqSpan seq_span(const SharedAttnArgs& a, int b) {
     SeqSpan s;
-    s.ctx = min(a.ctx_lens[b], a.max_ctx);
+    s.ctx = context_of(a, b);
     if (!a.starts) {
         s.t0 = b;
         s.n = 1;
@@ -94,8 +95,9 @@ __device__ __forceinline__ int seq_of(const SharedAttnArgs& a, int token) {
     }
     return a.starts[lo] <= token ? lo : -1;
 }
+// (positions may be negative and a window as large as the type: no difference is formed that leaves it)
 __device__ __forceinline__ int window_lo(const SharedAttnArgs& a, int pos) {
-    return a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
 }
 
 // The larger of this lane's value and the one lane ^ 32 holds: one v_permlane32_swap, no LDS round trip.
@@ -262,7 +264,7 @@ __device__ __forceinline__ void put_out(const SharedAttnArgs& a, int token, int 
 // Adds the weights of a sequence's own tokens that its only range has left logits of (from position 0 on); fin: every head's
 // maximum and inverse denominator.
 __device__ __forceinline__ void add_weights(const SharedAttnArgs& a, int b, int hk, const float (*fin)[2]) {
-    const int ctx = min(a.ctx_lens[b], a.max_ctx), lo = max(window_lo(a, ctx - 1), a.folded);
+    const int ctx = context_of(a, b), lo = max(window_lo(a, ctx - 1), a.folded);
     const float* x = a.logits + ((int64_t)b * a.Hq + hk * a.G) * a.lstride;
     for (int rel = lo / 4 * 4 + 4 * (int)threadIdx.x; rel < ctx; rel += 4 * SA_THREADS) {
         float* slot[4];
@@ -838,7 +840,7 @@ __device__ __forceinline__ void score_part(const SharedAttnArgs& a, int id, int 
     __shared__ float fin[HEADS][2];
     const int hk = id % a.Hkv, piece = id / a.Hkv % pieces, b = id / a.Hkv / pieces, tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ctx = min(a.ctx_lens[b], a.max_ctx), lo = window_lo(a, ctx - 1), first = a.prefix_len + piece * SA_SCORE_KEYS;
+    const int ctx = context_of(a, b), lo = window_lo(a, ctx - 1), first = a.prefix_len + piece * SA_SCORE_KEYS;
     if (first >= ctx || first + SA_SCORE_KEYS <= lo) return;
     const int rel = piece * SA_SCORE_KEYS + 4 * tid;
     const bool some = a.prefix_len + rel < ctx;

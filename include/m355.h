@@ -370,7 +370,7 @@ M355_API int m355_norm_qkv_rope_kv_write(const void* x_f16, const void* delta_f1
  * m355_attn_prefill, whose arithmetic (scale, sinks, window) they share.  dtype: M355_DTYPE_F16 or _BF16 for q, the caches,
  * sinks and out.  D 64 or 128, any Hq that is a multiple of Hkv, any page size.  Caches [num_blocks][block_size][Hkv][D],
  * pages block_stride elements apart (a multiple of 8); table entries outside [0, num_blocks) are clamped (no access leaves
- * the cache; such a result has no meaning).  ctx_lens count the new tokens and are clamped to max_ctx (host).
+ * the cache; such a result has no meaning).  ctx_lens count the new tokens and are clamped to 0 .. max_ctx (host).
  *
  * m355_shared_prefix_attn: new tokens q [T][Hq][D] (token stride q_stride) against the cache.  seq_starts [B + 1] (device):
  *   first tokens of the sequences, max_q (host) the longest one's number of tokens; NULL: one token per sequence (T == B).
