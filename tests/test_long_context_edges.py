@@ -4,7 +4,7 @@ layers whose graphs outlive a buffer.  Oracle and tolerances are those of test_l
 import pytest
 import torch
 
-from test_long_context import F16, Cache, _inputs, check, oracle, score_err
+from test_long_context import BF16, F16, Cache, _inputs, check, oracle, score_err
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -48,3 +48,63 @@ def test_gpu_negative_lengths_are_empty(P, window, m355, cuda):
     got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=P + 70, scale=0.125, window=window, seq_starts=st, max_q=5)
     check(got, want, mag, F16, score_err(c, q, 0.125))
     assert (got[2:6] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# weights far below the largest
+# ---------------------------------------------------------------------------------------------------------------------
+# fp16 probabilities: the largest of a row is held as 2^9 or more, so one that falls below the normal range is off by at
+# most half of 2^-24 of that, 2^-34 of the largest, on top of the relative half step that test_long_context.py counts.
+FP16_LOST = 2.0 ** -34
+
+# sequences, own tokens, new tokens, prefix, position of the dominant key, heads
+DOMINATED = [(64, 1500, 1, 0, 7, (4, 2)), (40, 3, 1, 6000, 11, (8, 2)), (3, 900, 1, 0, 899, (8, 2)), (4, 300, 300, 3000, 2999, (8, 2)),
+             (2, 256, 256, 1500, 3, (64, 8)), (1, 40, 7, 4096, 4000, (6, 2))]
+
+
+def _dominated(case, gap, dtype):
+    B, own, n, P, at, (Hq, Hkv) = DOMINATED[case]
+    c = Cache(900 + case, [P + own] * B, Hkv, 64, 16, dtype, prefix=P)
+    c.k[..., 0] = (0.05 * torch.randn(c.k.shape[:3], generator=c.g)).to(dtype)
+    c.v = (1 + 0.25 * torch.randn(c.v.shape, generator=c.g)).to(dtype)
+    for b in range(B):
+        page, off = c.slots(b)
+        c.k[page[at], off[at], :, 0] = gap
+        c.v[page[at], off[at]] = 0
+    c.k_norm = float(c.k.float().norm(dim=-1).max())
+    q = torch.zeros((B * n, Hq, 64), dtype=dtype)
+    q[..., 0] = 8                                              # scores, at a scale of 1/8, are the keys' first columns
+    return c, q, [n] * B
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gap", [12.0, 17.5, 20.0, 22.0])
+@pytest.mark.parametrize("case", range(len(DOMINATED)))
+def test_gpu_one_key_dominates(case, gap, dtype, m355, cuda):
+    """One key whose value is 0, thousands of others 12 to 22 nats below it: what they add up to is the output."""
+    c, q, n = _dominated(case, gap, dtype)
+    P, B = c.prefix, len(n)
+    want, mag, weights = oracle(c, q, n, 0.125)
+    rel = score_err(c, q, 0.125)
+    lost = FP16_LOST * 2.5 * max(c.ctx) if dtype == F16 else 0.0          # (values lie below 2.5)
+    kc, vc, bt, cl = c.device(cuda)
+    assert float(c.v.abs().max()) < 2.5
+    st = None if n[0] == 1 else torch.arange(0, B * n[0] + 1, n[0], dtype=torch.int32, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125, seq_starts=st, max_q=n[0])
+    _check_lost(got, want, mag, dtype, rel, lost)
+    if n[0] == 1:
+        sc = torch.zeros(c.scores.shape, device=cuda)
+        got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125)
+        _check_lost(got, want, mag, dtype, rel, lost)
+        for b in range(B):
+            page, off = c.slots(b)
+            w = weights[b].t()[P:]
+            assert ((sc.cpu().double()[page[P:], :, off[P:]] - w).abs() <= (2 * rel + 2.0 ** -23 * (q.shape[1] // c.Hkv)) * w).all()
+
+
+def _check_lost(got, want, mag, dtype, rel, lost):
+    half = torch.finfo(dtype).eps / 2
+    tol = half * want.abs() + (half + 2 * rel) * mag + 2 * torch.finfo(dtype).smallest_normal * half + lost
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f} of the tolerance"
