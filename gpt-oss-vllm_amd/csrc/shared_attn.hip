@@ -475,11 +475,13 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         // The exponents' reference follows the running maximum lazily: probabilities are formed against the old one, and only
         // if one of them exceeds LIMIT (seen on the packed 16-bit values, whose order is that of whole numbers) do the maximum,
         // the rescaling and the probabilities take another turn: a few times per row instead of a maximum per tile.  The
-        // denominator carries the same factor.  bf16 has the exponents of fp32.  fp16 ends at 2^-24 below and 65504 above, so its
+        // denominator carries the same factor.  fp16 ends at 2^-24 below and 65504 above, so its
         // reference is put 2^LIFT below the maximum: a row's largest probability is held as 2^9 to 2^16, and one that falls
         // out of the normal range is off by at most 2^-34 of the largest (2^-25 with the maximum itself as the reference, which
         // lost thousands of keys 18 nats below one that dominates).  A higher lift leaves less room before the next turn: 2^9
-        // costs nothing, 2^10 1 %, 2^11 4 % (32 tokens on 8192, drafted tokens, prompts).
+        // costs nothing, 2^10 1 %, 2^11 4 % (32 tokens on 8192, drafted tokens, prompts).  bf16 has the exponents of fp32, its
+        // values too: there the reference lies above the maximum, so that no probability exceeds 2^-16 and 65536 of them times
+        // the largest finite value still add up to a finite sum.
         uint32_t pb[QT][8];
         float sum[QT];
         auto exponentials = [&] {
@@ -501,8 +503,8 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             return top;
         };
         const ushort2_t top = exponentials();
-        constexpr uint16_t LIMIT = __is_same(E, half_t) ? 0x7bffu : 0x4580u;   // 65504, 2^12
-        constexpr float LIFT = __is_same(E, half_t) ? 9.f : 0.f;
+        constexpr uint16_t LIMIT = __is_same(E, half_t) ? 0x7bffu : 0x3780u;   // 65504, 2^-16
+        constexpr float LIFT = __is_same(E, half_t) ? 9.f : -28.f;
         if (__any(top[0] > LIMIT || top[1] > LIMIT)) {
 #pragma unroll
             for (int q = 0; q < QT; q++) {

@@ -108,3 +108,29 @@ def _check_lost(got, want, mag, dtype, rel, lost):
     tol = half * want.abs() + (half + 2 * rel) * mag + 2 * torch.finfo(dtype).smallest_normal * half + lost
     err = (got.cpu().double() - want).abs()
     assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f} of the tolerance"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,own,n,P,heads", [(1, 700, 1, 0, (4, 2)), (40, 5, 1, 3000, (8, 2)), (1, 300, 300, 1000, (8, 2)), (2, 256, 256, 1500, (64, 8)),
+                                             (1, 5000, 1, 0, (33, 1))])
+def test_gpu_values_near_the_largest_finite_ones(B, own, n, P, heads, m355, cuda):
+    """bfloat16 values of up to 2^126 and scores that grow along the keys by as much as leaves the reference where it was:
+    the output is an average of the values, however large its terms were on the way."""
+    Hq, Hkv = heads
+    c = Cache(950, [P + own] * B, Hkv, 64, 16, BF16, prefix=P)
+    for b in range(B):
+        page, off = c.slots(b)
+        c.k[page, off, :, 0] = (7.5 * torch.arange(c.ctx[b]) / c.ctx[b]).to(BF16)[:, None]     # 2^10.8 from the first to the last
+    c.v = (c.v.float().clamp(-4, 4) * 2.0 ** 124).to(BF16)
+    c.k_norm = float(c.k.float().norm(dim=-1).max())
+    q = torch.zeros((B * n, Hq, 64), dtype=BF16)
+    q[..., 0] = 8
+    want, mag, _ = oracle(c, q, [n] * B, 0.125)
+    kc, vc, bt, cl = c.device(cuda)
+    st = None if n == 1 else torch.arange(0, B * n + 1, n, dtype=torch.int32, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125, seq_starts=st, max_q=n)
+    check(got, want, mag, BF16, score_err(c, q, 0.125))
+    if n == 1:
+        got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, torch.zeros(c.scores.shape, device=cuda), bt, cl, prefix_len=P, max_ctx=max(c.ctx),
+                                            scale=0.125)
+        check(got, want, mag, BF16, score_err(c, q, 0.125))
