@@ -208,6 +208,9 @@ __device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t a2, u
         : "memory");
 }
 
+// A factor between reference points that never underflows to 0: an infinite or NaN value behind it stays what it is.
+__device__ __forceinline__ float factor(float from, float to) { return from == to ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-149f); }
+
 // The ranges of one row, lane i looking after range i0 + i: does the row see a key of it (else nothing was written), and
 // its (m, l).
 struct RangeStat {
@@ -235,17 +238,17 @@ __device__ __forceinline__ void start_with_sink(const SharedAttnArgs& a, int hea
         den = sk == -INFINITY ? 0.f : sk == sk ? 1.0f : sk;   // (a NaN stays one)
     }
 }
-// One step of the running (m, den) over the ranges of N neighbouring lanes: returns this lane's factor (0: leave its range
-// out).
+// One step of the running (m, den) over the ranges of N neighbouring lanes: returns this lane's factor (0: its range was not
+// written).
 template <int N>
 __device__ __forceinline__ float join_stats(const RangeStat& s, float& m_run, float& den, float& back) {
     float top = s.m;
 #pragma unroll
     for (int o = 1; o < N; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float m_new = fmaxf(m_run, top);
-    back = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-    const float f = !s.live || s.l == 0.f ? 0.f : s.m == m_new ? 1.0f : __builtin_amdgcn_exp2f(s.m - m_new);
-    float part = f == 0.f && s.l == s.l ? 0.f : f * s.l;
+    back = factor(m_run, m_new);
+    const float f = s.live ? factor(s.m, m_new) : 0.f;
+    float part = f * s.l;   // (not written: l is 0)
 #pragma unroll
     for (int o = 1; o < N; o *= 2) part += __shfl_xor(part, o, 64);
     den = den * back + part;
@@ -608,6 +611,44 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                 *reinterpret_cast<float4_t*>(at + qi * D * 4 + (((8 * dt + 2 * i4 + hh) ^ (qi & 15)) << 4)) =
                     float4_t{acc[dt][4 * i4], acc[dt][4 * i4 + 1], acc[dt][4 * i4 + 2], acc[dt][4 * i4 + 3]};
     };
+    // An output may be NaN only because an infinite value met a probability that rounds to 0: then the values of that column
+    // that the row sees are looked through once more (tiles that are seen in part count them in the walk).
+    auto settle = [&](unsigned char* at, const f32x16_t(&acc)[DT], float l, int row_pos, int row_lo) {
+        float z[4] = {0.f, 0.f, 0.f, 0.f};   // (0 times an infinity or NaN: one instruction per value)
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[i & 3] = __builtin_fmaf(acc[dt][i], 0.f, z[i & 3]);
+        if (!__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f)) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int i = 0; i < 32 * CH / 64; i++) {
+            const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+            const int first = max(kfloor, __shfl(row_lo, r, 64)), last = min(kend - 1, __shfl(row_pos, r, 64));
+            const float lr = __shfl(l, r, 64);
+            float4_t* to = reinterpret_cast<float4_t*>(at + r * D * 4 + ((c ^ (r & 15)) << 4));
+            float4_t v = *to;
+            uint32_t asked = 0, plus = 0, minus = 0;   // bit e: column 4 c + e
+#pragma unroll
+            for (int e = 0; e < 4; e++) asked |= lr == lr && v[e] != v[e] ? 1u << e : 0u;   // (l is NaN where a score is)
+            for (int key = first; key <= last && (plus & minus & asked) != asked; key++) {
+                const int page = page_of(a, key), blk = min(max(key < folded ? a.tables[page] : table[page], 0), a.num_blocks - 1);
+                const int64_t off = blk * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D + 4 * c;
+                const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const E*>(a.vc) + off);
+                u32x4_t clean, p, m;
+                if (split_nonfinite<E>(u32x4_t{raw[0], raw[1], 0u, 0u}, clean, p, m))
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        plus |= (p[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 1u << e : 0u;
+                        minus |= (m[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 1u << e : 0u;
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (asked & (plus ^ minus) & 1u << e) v[e] = plus >> e & 1 ? INFINITY : -INFINITY;
+            *to = v;
+        }
+    };
     auto get = [&](const unsigned char* at, int r, int c) { return *reinterpret_cast<const float4_t*>(at + r * D * 4 + ((c ^ (r & 15)) << 4)); };
     if constexpr (RW == 4) {
         static_assert(SA_WAVES * 32 * D * 4 <= W::TILES);
@@ -617,6 +658,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         for (int q = 0; q < QT; q++) {
             put(at, o[q]);
             const float l = half_sum(l_run[q]);
+            settle(at, o[q], l, pos[q], lo[q]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const int first = row0 + 32 * (wave * QT + q), c = lane % CH;
             if (direct) {
@@ -628,7 +670,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                     const int r32 = i * (64 / CH) + lane / CH, rr = first + r32;
                     const float fr = __shfl(f, r32, 64), ir = __shfl(inv, r32, 64);
                     const float4_t v = get(at, r32, c);
-                    if (rr < row_end) put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, fr != 0.f ? fr * v : float4_t{0.f, 0.f, 0.f, 0.f}, ir);
+                    if (rr < row_end) put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, fr * v, ir);
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 continue;
@@ -651,6 +693,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
         put(tiles, o[0]);   // (each wave in place of its own tile)
         const float lsum = half_sum(l_run[0]);
+        settle(tiles, o[0], lsum, pos[0], lo[0]);
         if (hh == 0) {
             wm[wave][qi] = m_run[0];
             wl[wave][qi] = lsum;
@@ -665,7 +708,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 #pragma unroll
                     for (int w = 1; w < SA_WAVES; w++) m = fmaxf(m, wm[w][tid]);
 #pragma unroll
-                    for (int w = 0; w < SA_WAVES; w++) l += (wm[w][tid] == m ? 1.0f : __builtin_amdgcn_exp2f(wm[w][tid] - m)) * wl[w][tid];
+                    for (int w = 0; w < SA_WAVES; w++) l += factor(wm[w][tid], m) * wl[w][tid];
                     start_with_sink<E>(a, hk * a.G + tid, m_all, den);
                     join_stats<1>(RangeStat{true, m, l}, m_all, den, back);
                     fin[tid][0] = m_all;
@@ -684,7 +727,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < SA_WAVES; w++) {
-                const float f = wm[w][r32] == m ? 1.0f : __builtin_amdgcn_exp2f(wm[w][r32] - m);   // (nothing seen at all: 1 * 0)
+                const float f = factor(wm[w][r32], m);   // (nothing seen at all: 1 * 0)
                 tot += f * get(smem + w * W::NS * W::STAGE, r32, c);
                 l += f * wl[w][r32];
             }
@@ -693,7 +736,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                 float m_all, den, back;
                 start_with_sink<E>(a, hk * a.G + rr % a.G, m_all, den);
                 const float f = join_stats<1>(RangeStat{true, m, l}, m_all, den, back);
-                put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, f != 0.f ? f * tot : float4_t{0.f, 0.f, 0.f, 0.f}, inverse(den));
+                put_out<E>(a, rr / a.G, hk * a.G + rr % a.G, D, c, f * tot, inverse(den));
                 continue;
             }
             const int64_t r = split * rows + (int64_t)(rr / a.G) * a.Hq + hk * a.G + rr % a.G;

@@ -379,7 +379,7 @@ M355_API int m355_norm_qkv_rope_kv_write(const void* x_f16, const void* delta_f1
  *   read through row 0 of block_tables (once for all, where that is cheaper than again for every sequence), the others through
  *   the sequence's own row.  prefix_len need not end a page.  Queries may lie anywhere (a prefix_len beyond a sequence's end only hides what it does not see).  Rows that see
  *   nothing become 0; rows of q behind seq_starts[B], and a sequence's tokens behind max_q, leave `out` as it was.
- *   Infinities and NaN in K or V reach the queries that see them and no others.
+ *   Infinities and NaN in K or V reach the queries that see them, however little their key weighs, and no others.
  *   With one sequence per row and prefix_len = 0 it is m355_paged_attn_decode_ex.
  */
 M355_API int m355_shared_prefix_attn(const void* q, const void* kcache, const void* vcache, const int32_t* block_tables,

@@ -79,8 +79,7 @@ def _dominated(case, gap, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("gap", [12.0, 17.5, 20.0, 22.0])
-@pytest.mark.parametrize("case", range(len(DOMINATED)))
+@pytest.mark.parametrize("case, gap", [(c, g) for c in range(len(DOMINATED)) for g in ((17.5, 20.0) if c == 4 else (12.0, 17.5, 20.0, 22.0))])
 def test_gpu_one_key_dominates(case, gap, dtype, m355, cuda):
     """One key whose value is 0, thousands of others 12 to 22 nats below it: what they add up to is the output."""
     c, q, n = _dominated(case, gap, dtype)
@@ -134,3 +133,77 @@ def test_gpu_values_near_the_largest_finite_ones(B, own, n, P, heads, m355, cuda
         got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, torch.zeros(c.scores.shape, device=cuda), bt, cl, prefix_len=P, max_ctx=max(c.ctx),
                                             scale=0.125)
         check(got, want, mag, BF16, score_err(c, q, 0.125))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# infinite and NaN values that weigh almost nothing
+# ---------------------------------------------------------------------------------------------------------------------
+def _same_nonfinite(got, want, mag, dtype, rel, lost):
+    got = got.cpu().double()
+    bad = ~want.isfinite()
+    assert torch.equal(got.isfinite(), ~bad)
+    assert torch.equal(got[bad].isnan(), want[bad].isnan()) and torch.equal(got[got.isinf()], want[want.isinf()])
+    zero = torch.zeros_like(want)
+    _check_lost(torch.where(bad, zero, got), torch.where(bad, zero, want), torch.where(bad, zero, mag), dtype, rel, lost)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("by", ["key", "sink"])
+@pytest.mark.parametrize("case, gap", [(c, g) for c in range(len(DOMINATED)) for g in ((30.0, 110.0) if c == 4 else (14.0, 30.0, 110.0, 250.0))])
+def test_gpu_nonfinite_values_of_keys_that_weigh_nothing(case, by, gap, dtype, m355, cuda):
+    """Infinite and NaN values of keys 14 to 250 nats below a dominating key, or below the sink, reach every query that sees
+    them, as what they are: next to the dominating key, in the same range, in other ranges, in the prefix and behind it."""
+    c, q, n = _dominated(case, gap if by == "key" else 0.0, dtype)
+    sinks = torch.full((q.shape[1],), gap).to(dtype) if by == "sink" else None
+    P, B, at, ctx = c.prefix, len(n), DOMINATED[case][4], c.ctx[0]
+    near = at + 1 if at + 1 < ctx else at - 1
+    spots = [(near, 1, float("nan")), (near, 2, float("inf")), (ctx // 2, 5, float("-inf")), (ctx // 2, 6, float("nan")), (0, 63, float("inf")),
+             (ctx - 1, 33, float("inf")), (max(P - 1, 2), 40, float("-inf")), (ctx // 3, 12, float("inf")), (ctx // 5, 12, float("inf")),
+             (ctx // 3, 13, float("inf")), (ctx // 5, 13, float("-inf"))]
+    for pos, column, value in spots:
+        if pos != at:
+            for b in range(B if pos >= P else 1):
+                page, off = c.slots(b)
+                c.v[page[pos], off[pos], c.Hkv - 1, column] = value            # (the other KV heads stay finite)
+    want, mag, _ = oracle(c, q, n, 0.125, sinks)
+    assert want.isnan().any() and want.isinf().any() and want.isfinite().any()
+    rel = score_err(c, q, 0.125)
+    lost = FP16_LOST * 2.5 * max(c.ctx) if dtype == F16 else 0.0
+    kc, vc, bt, cl = c.device(cuda)
+    st = None if n[0] == 1 else torch.arange(0, B * n[0] + 1, n[0], dtype=torch.int32, device=cuda)
+    sk = None if sinks is None else sinks.to(cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=ctx, scale=0.125, seq_starts=st, max_q=n[0], sinks=sk)
+    _same_nonfinite(got, want, mag, dtype, rel, lost)
+    if n[0] == 1:
+        sc = torch.zeros(c.scores.shape, device=cuda)
+        got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, prefix_len=P, max_ctx=ctx, scale=0.125, sinks=sk)
+        _same_nonfinite(got, want, mag, dtype, rel, lost)
+        assert sc.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 700])
+def test_gpu_nonfinite_keys_and_queries(window, m355, cuda):
+    """A NaN in a key or in a query reaches the rows whose scores it enters, whatever their other weights, and no other."""
+    P, n = 2500, [3, 1]
+    c = Cache(77, [P + 40, P + 9], 2, 64, 16, F16, prefix=P)
+    q, _ = _inputs(c, 4, 16, 3, False)
+    rel = score_err(c, q, 0.125)
+    want, mag, _ = oracle(c, q, n, 0.125, window=window)
+    page, off = c.slots(0)
+    c.k[page[P + 38], off[P + 38], 0, 5] = float("nan")          # rows 1 and 2 of the first sequence see it, KV head 0
+    c.k[page[P - 660], off[P - 660], 1, 9] = float("nan")        # windowed: rows 0 (and 3) see it, KV head 1; else everyone
+    q[3, 15, 7] = float("nan")
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool)
+    hit[1:3, :8] = True
+    for row, pos in ((0, P + 37), (1, P + 38), (2, P + 39), (3, P + 8)):
+        if not window or P - 660 > pos - window:
+            hit[row, 8:] = True
+    hit[3, 15] = True
+    kc, vc, bt, cl = c.device(cuda)
+    st = torch.tensor([0, 3, 4], dtype=torch.int32, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=P + 40, scale=0.125, seq_starts=st, max_q=3, window=window).cpu()
+    assert got[hit].isnan().all()
+    zero = torch.zeros_like(want)
+    check(torch.where(hit[..., None], torch.zeros_like(got), got), torch.where(hit[..., None], zero, want), mag, F16, rel)
