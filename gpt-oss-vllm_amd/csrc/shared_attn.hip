@@ -23,6 +23,7 @@
 // ahead, four or five tiles in LDS instead of three.  Few tokens: launches (7 us for one, 10 for the ranges and their joining).
 #include "common.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -991,11 +992,11 @@ static double cut_cost(int64_t keys, int64_t units, const CutCost& w, int64_t le
     return 7000 + len * (per_key > w.alone ? per_key : w.alone) + w.start * c + w.merge * used +
            w.uneven * w.alone * len / (c + w.others < 1 ? 1 : c + w.others) + 0.5 * behind * w.beside;
 }
-static double cut_keys(int64_t keys, int64_t units, const CutCost& w, int& n, int& len) {
+static double cut_keys(int64_t keys, int64_t units, const CutCost& w, int64_t most, int& n, int& len) {
     n = 0, len = 128;
     if (keys <= 0) return 0;
     double best = 0;
-    for (int64_t k = 1; k <= 1024 && (k == 1 || (k - 1) * 128 < keys); k += k < 16 ? 1 : k / 8) {
+    for (int64_t k = 1; k <= 1024 && (k == 1 || k <= most) && (k == 1 || (k - 1) * 128 < keys); k += k < 16 ? 1 : k / 8) {
         const int64_t l = ((keys + k - 1) / k + 127) / 128 * 128;
         const double t = cut_cost(keys, units, w, l);
         if (n == 0 || t < best) best = t, n = (int)((keys + l - 1) / l), len = (int)l;
@@ -1007,9 +1008,13 @@ struct SharedAttnPlan {
     bool direct;                 // one range, which takes the prefix along
     int prefix_rows, own_rows;   // rows per workgroup: 32 (RW = 1), 128 or 256 (RW = 4)
     int64_t units;               // an upper bound of every launch's workgroups and row numbers
-    size_t part_floats, logit_floats, bytes;
+    size_t part_floats, bytes;   // the workspace: ranges' outputs, then (scored) logits; of both
+    size_t least;                // a workspace of so many bytes will do
 };
-static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, int window, bool scored) {
+// The cheapest plan that makes do with a workspace of `budget` bytes (at least `least`, which no smaller call exceeds: a
+// workspace that was made for the largest call serves all of them, with fewer ranges where the best number does not fit).
+static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, int window, bool scored,
+                                       size_t budget) {
     SharedAttnPlan p;
     max_q = max_q < T ? max_q : T;
     const int64_t G = Hq / Hkv, P = prefix_len < max_ctx ? prefix_len : max_ctx, own = max_ctx - P, R = T * G;
@@ -1029,8 +1034,21 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
         return w;
     };
     const int64_t own_units = Hkv * (int64_t)B * ((max_q * G + p.own_rows - 1) / p.own_rows);
-    double t = cut_keys(P, prefix_units, cost(false, p.prefix_rows, p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0), p.np, p.sp);
-    t += cut_keys(own, own_units, cost(true, p.own_rows, 0), p.ns, p.so) - (P && own > 0 ? 7000 : 0);
+    const size_t rows = (size_t)T * Hq, range = rows * (D + 2);   // floats that a range leaves behind
+    auto logits_of = [&](int64_t keys) { return scored ? rows * (size_t)((keys + 127) / 128 * 128) : (size_t)0; };
+    auto cut = [&](int64_t most_p, int64_t most_s) {
+        const double prefix = cut_keys(P, prefix_units, cost(false, p.prefix_rows, p.own_rows == 32 ? (double)own * B * Hkv * D * 4 / 5000 : 0), most_p, p.np, p.sp);
+        return prefix + cut_keys(own, own_units, cost(true, p.own_rows, 0), most_s, p.ns, p.so) - (P && own > 0 ? 7000 : 0);
+    };
+    p.least = scored ? (2 * range + logits_of(own) + 4) * sizeof(float) : 256;
+    double t = cut(1024, 1024);
+    const size_t room = budget / sizeof(float) > logits_of(own) ? budget / sizeof(float) - logits_of(own) : 0;
+    const int64_t fit = (int64_t)(room / 4 * 4 / range);   // ranges that there is room for
+    const bool ranges = fit >= (P > 0) + (own > 0);
+    if (ranges && p.np + p.ns > fit) {   // (as many for the prefix as its share of the best plan)
+        const int64_t most_p = P ? (own > 0 ? std::min<int64_t>(std::max<int64_t>(p.np * fit / (p.np + p.ns), 1), fit - 1) : fit) : 0;
+        t = cut(most_p, fit - most_p);
+    }
     // One range per sequence, which takes the prefix along, instead: every sequence reads the prefix again (from the L2s), but
     // no outputs are left to be joined, nor is there a second launch (about 3000 ns of the host's time, and a base of 5500 for 7000).
     // Fitted to 31 pairs, among them (us of kernels, ranges and joining / one range): 4 sequences of 200 + 33 tokens 9.6 / 7.2,
@@ -1052,16 +1070,14 @@ static SharedAttnPlan plan_shared_attn(int T, int B, int max_q, int Hq, int Hkv,
         p.prefix_rows = p.own_rows;   // (no kernel with more LDS and registers than the own walks use)
     };
     p.direct = false;
-    if ((!scored || G <= 32) && one_range(P, own) < t + 3000) take_one_range();
-    const size_t rows = (size_t)T * Hq;
-    p.part_floats = ((size_t)(p.np + p.ns) * rows * (D + 2) + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
-    p.lstride = (int)(((p.direct ? max_ctx : own) + 127) / 128 * 128);
-    p.logit_floats = scored ? rows * (size_t)p.lstride : 0;
-    p.bytes = (p.part_floats + p.logit_floats) * sizeof(float);
+    if ((!scored || (G <= 32 && logits_of(max_ctx) * sizeof(float) <= budget)) && (!ranges || one_range(P, own) < t + 3000)) take_one_range();
     if (window > 0 && !scored && !p.direct) {   // (a row set sees its queries' positions and the window in front of the first)
         const int64_t seen = (int64_t)window + (p.own_rows == 32 ? max_q : 128 / G + 1);
         if (seen < max_ctx && one_range(0, seen) < t + 3000) take_one_range();
     }
+    p.part_floats = p.direct ? 0 : ((size_t)(p.np + p.ns) * range + 3) / 4 * 4;   // (the logits behind it are stored 16 bytes at a time)
+    p.lstride = (int)(((p.direct ? max_ctx : own) + 127) / 128 * 128);
+    p.bytes = (p.part_floats + logits_of(p.direct ? max_ctx : own)) * sizeof(float);
     p.units = (int64_t)Hq * T * (p.np + 1) + (int64_t)Hkv * B * (p.ns * (max_q * G / 32 + 1) + own / SA_SCORE_KEYS + 1);
     return p;
 }
@@ -1094,6 +1110,22 @@ static int launch_shared_attn(SharedAttnArgs& a, const SharedAttnPlan& p, bool s
     return 0;
 }
 
+// What a workspace is asked to hold: twice the ranges of the best plan (up to 32 MB more) and of the best ones for fewer tokens
+// (down to single ones, by factors of four), since a call with fewer tokens or a shorter context often wants more of them, and
+// it is made once for the largest call.  By the model, 0.3 % of 300000 random pairs of a largest and a smaller call then take
+// another plan than with all the memory they want, 0.15 % at a cost of more than 15 %.
+static size_t shared_attn_workspace(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len, bool scored) {
+    size_t need = 0;
+    auto ask = [&](int t, int b, int n) {
+        const SharedAttnPlan p = plan_shared_attn(t, b, n, Hq, Hkv, D, max_ctx, prefix_len, 0, scored, SIZE_MAX);
+        need = std::max({need, p.least, p.bytes + std::min<size_t>(p.part_floats * sizeof(float), 32 << 20)});
+    };
+    for (int t = T; t > 0; t /= 4) ask(t, std::min(B, t), std::min(max_q, t));
+    if (max_q > 1)
+        for (int t = std::min(T, B); t > 0; t /= 4) ask(t, t, 1);
+    return need;
+}
+
 // What both entry points check and set up alike.  Returns 0 with `a` and `p` filled in.
 static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan& p, const void* q, const void* kc, const void* vc,
                              const int32_t* tables, const int32_t* ctx_lens, const int32_t* starts, int T, int B, int max_q, int Hq,
@@ -1115,10 +1147,11 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     if (q_stride < (int64_t)Hq * D || o_stride < (int64_t)Hq * D || q_stride % 8)
         return fail(-2, "%s: token strides must cover the heads, q's be a multiple of 8 elements", who);
     if (!aligned(q, 16) || !aligned(kc, 16) || !aligned(vc, 16)) return fail(-3, "%s: q and caches must be 16-byte aligned", who);
-    p = plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, window, scored);
+    p = plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, window, scored, ws_bytes);
     if (max_ctx > (1 << 30) || p.units >= (1ll << 30))
         return fail(-2, "%s: unsupported size T=%d B=%d max_q=%d Hq=%d max_ctx=%d", who, T, B, max_q, Hq, max_ctx);
-    if (!workspace || ws_bytes < p.bytes) return fail(-6, "%s: workspace of %zu bytes needed, %zu given", who, p.bytes, ws_bytes);
+    if (!workspace || ws_bytes < p.least || ws_bytes < p.bytes)
+        return fail(-6, "%s: workspace of %zu bytes needed, %zu given", who, std::max(p.least, p.bytes), ws_bytes);
     if (!aligned(workspace, 16)) return fail(-3, "%s: the workspace must be 16-byte aligned", who);
     a = SharedAttnArgs{};
     a.q = q, a.kc = kc, a.vc = vc, a.sinks = sinks, a.tables = tables, a.ctx_lens = ctx_lens, a.starts = starts;
@@ -1132,8 +1165,10 @@ static int setup_shared_attn(const char* who, SharedAttnArgs& a, SharedAttnPlan&
     a.np = p.np, a.sp = p.sp, a.ns = p.ns, a.so = p.so;
     a.direct = p.direct;
     if (p.direct) a.folded = a.prefix_len, a.prefix_len = 0;
-    a.part_o = reinterpret_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)(p.np + p.ns) * T * Hq * D;
+    if (!p.direct) {
+        a.part_o = reinterpret_cast<float*>(workspace);
+        a.part_ml = a.part_o + (size_t)(p.np + p.ns) * T * Hq * D;
+    }
     a.out = out;
     return 0;
 }
@@ -1144,12 +1179,12 @@ using namespace m355;
 
 extern "C" size_t m355_shared_prefix_attn_workspace_bytes(int T, int B, int max_q, int Hq, int Hkv, int D, int max_ctx, int prefix_len) {
     if (T <= 0 || B <= 0 || max_q <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_ctx <= 0 || prefix_len < 0) return 0;
-    return plan_shared_attn(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, 0, false).bytes;
+    return shared_attn_workspace(T, B, max_q, Hq, Hkv, D, max_ctx, prefix_len, false);
 }
 
 extern "C" size_t m355_paged_attn_decode_scored_workspace_bytes(int B, int Hq, int Hkv, int D, int max_ctx, int prefix_len) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_ctx <= 0 || prefix_len < 0) return 0;
-    return plan_shared_attn(B, B, 1, Hq, Hkv, D, max_ctx, prefix_len, 0, true).bytes;
+    return shared_attn_workspace(B, B, 1, Hq, Hkv, D, max_ctx, prefix_len, true);
 }
 
 extern "C" int m355_shared_prefix_attn(const void* q, const void* kcache, const void* vcache, const int32_t* block_tables,
@@ -1182,7 +1217,7 @@ extern "C" int m355_paged_attn_decode_scored(const void* q, const void* kcache, 
                                    D, dtype, num_blocks, block_size, max_blocks, block_stride, max_ctx, prefix_len, q_stride, o_stride, scale,
                                    sinks, window, true, workspace, ws_bytes, out))
         return rc;
-    a.logits = a.part_o + p.part_floats;
+    a.logits = reinterpret_cast<float*>(workspace) + p.part_floats;
     a.lstride = p.lstride;
     a.scores = scores;
     hipStream_t st = (hipStream_t)stream;

@@ -381,6 +381,10 @@ M355_API int m355_norm_qkv_rope_kv_write(const void* x_f16, const void* delta_f1
  *   nothing become 0; rows of q behind seq_starts[B], and a sequence's tokens behind max_q, leave `out` as it was.
  *   Infinities and NaN in K or V reach the queries that see them, however little their key weighs, and no others.
  *   With one sequence per row and prefix_len = 0 it is m355_paged_attn_decode_ex.
+ *   workspace: m355_shared_prefix_attn_workspace_bytes of this call, or of one with no fewer tokens, sequences, new tokens per
+ *   sequence and cached tokens (prefix_len as here, or 0): made once for the largest call it serves all of them.  A call that
+ *   would like more than it is given takes fewer ranges of keys (the order of the sums, and so the last bits of the output,
+ *   follow them).  The same holds for the scored form.
  */
 M355_API int m355_shared_prefix_attn(const void* q, const void* kcache, const void* vcache, const int32_t* block_tables,
                                      const int32_t* ctx_lens, const int32_t* seq_starts, int T, int B, int max_q, int Hq,

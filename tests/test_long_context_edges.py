@@ -207,3 +207,87 @@ def test_gpu_nonfinite_keys_and_queries(window, m355, cuda):
     assert got[hit].isnan().all()
     zero = torch.zeros_like(want)
     check(torch.where(hit[..., None], torch.zeros_like(got), got), torch.where(hit[..., None], zero, want), mag, F16, rel)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# workspaces
+# ---------------------------------------------------------------------------------------------------------------------
+def _answer(m355, ws_bytes, T, B, max_q, Hq, Hkv, D, max_ctx, prefix, scored):
+    """The call's answer to a workspace of so many bytes: -6 where it is too small, else -3, since it is at an odd address."""
+    ptr, L = 0x10000, m355.load()
+    blocks = (max_ctx + 15) // 16
+    tail = [16, blocks, 16 * Hkv * D, max_ctx, prefix, Hq * D, Hq * D, 0.1, None, 0, ptr + 1, ws_bytes, ptr, None]
+    if scored:
+        return L.m355_paged_attn_decode_scored(*[ptr] * 6, B, Hq, Hkv, D, 0, blocks, *tail)
+    return L.m355_shared_prefix_attn(*[ptr] * 6, T, B, max_q, Hq, Hkv, D, 0, blocks, *tail)
+
+
+def _need(m355, T, B, max_q, Hq, Hkv, D, max_ctx, prefix, scored):
+    if scored:
+        return m355.paged_attn_decode_scored_workspace_bytes(B, Hq, Hkv, D, max_ctx, prefix)
+    return m355.shared_prefix_attn_workspace_bytes(T, B, max_q, Hq, Hkv, D, max_ctx, prefix)
+
+
+@pytest.mark.parametrize("scored", [False, True])
+def test_a_workspace_for_the_largest_call_serves_every_smaller_one(scored, m355):
+    """Fewer tokens, sequences, cached tokens: no call asks for more than the largest one, although the numbers of ranges
+    that are best for them do.  Asked for without a prefix, it serves every prefix."""
+    import random
+    rng = random.Random(5)
+    fixed = [((32, 1, 64, 8, 64, 2300, 2048), (31, 1, 2300)), ((32, 1, 64, 8, 64, 2180, 2048), (32, 1, 2116)), ((32, 1, 64, 8, 64, 2116, 2048), (32, 1, 2100)),
+             ((96, 1, 32, 8, 128, 21035, 20011), (1, 1, 20012)), ((6, 400, 64, 8, 64, 8612, 8192), (1, 1, 8193)), ((4, 1, 130, 1, 64, 300, 200), (1, 1, 201))]
+    pairs = [(big, small) for big, small in fixed if not scored or big[1] == 1]
+    for _ in range(3000):
+        Hkv = rng.choice([1, 2, 4, 8])
+        P = rng.choice([0, rng.randint(1, 200), rng.randint(1, 20000)])
+        big = (rng.randint(1, 96), 1 if scored else rng.choice([1, rng.randint(2, 200)]), Hkv * rng.choice([1, 2, 5, 8, 33]), Hkv, rng.choice([64, 128]),
+               P + rng.randint(1, rng.choice([100, 1000, 30000])), P)
+        pairs.append((big, (rng.randint(1, big[0]), rng.randint(1, big[1]), rng.randint(1, big[5]))))
+    for (B, n, Hq, Hkv, D, ctx, P), (b, k, c) in pairs:
+        for asked in (P, 0):
+            ws = _need(m355, B * n, B, n, Hq, Hkv, D, ctx, asked, scored)
+            case = ((B, n, Hq, Hkv, D, ctx, P), (b, k, c), asked, ws)
+            assert _answer(m355, ws, B * n, B, n, Hq, Hkv, D, ctx, P, scored) == -3, case
+            assert _answer(m355, ws, b * k, b, k, Hq, Hkv, D, c, P, scored) == -3, case
+    # one range per sequence leaves nothing to join: a call that is best served by it asks for next to nothing
+    assert scored or _need(m355, 4, 4, 1, 64, 8, 64, 233, 200, False) <= 4096
+
+
+WORKSPACES = [([2000, 7, 300], [1, 1, 1], 0, (64, 8)), ([30, 1, 9], [1, 1, 1], 5000, (16, 2)), ([900, 40], [1, 1], 2100, (8, 2)),
+              ([700, 90], [5, 90], 3001, (16, 2)), ([300, 2], [1, 1], 130, (66, 1))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case, scored", [(i, s) for i in range(len(WORKSPACES)) for s in (False, True) if not s or max(WORKSPACES[i][1]) == 1])
+def test_gpu_results_hold_for_every_workspace(case, scored, m355, cuda):
+    """From the least that is accepted to all that is asked for: the same results within the tolerance, nothing written
+    behind the bytes that were named, nothing read that the call has not written."""
+    own, n, P, (Hq, Hkv) = WORKSPACES[case]
+    c = Cache(61, [P + o for o in own], Hkv, 64, 16, F16, prefix=P, n=n)
+    T, B, max_ctx = sum(n), len(n), P + max(own)
+    q, sk = _inputs(c, T, Hq, 6, True)
+    want, mag, weights = oracle(c, q, n, 0.125, sk)
+    kc, vc, bt, cl = c.device(cuda)
+    need = _need(m355, T, B, max(n), Hq, Hkv, 64, max_ctx, P, scored)
+    low, least = 0, need                       # the least that is accepted, by halving
+    while least - low > 4:
+        mid = (low + least) // 8 * 4
+        low, least = (low, mid) if _answer(m355, mid, T, B, max(n), Hq, Hkv, 64, max_ctx, P, scored) == -3 else (mid, least)
+    buffer = torch.empty(need + 4096, dtype=torch.uint8, device=cuda)
+    st = None if max(n) == 1 else torch.tensor([0] + [sum(n[:i + 1]) for i in range(B)], dtype=torch.int32, device=cuda)
+    rel = score_err(c, q, 0.125)
+    for part in range(9):
+        size = least + (need - least) * part // 8 // 4 * 4
+        buffer.fill_(255)
+        kw = dict(prefix_len=P, max_ctx=max_ctx, scale=0.125, sinks=sk.to(cuda), workspace=buffer[:size])
+        if scored:
+            sc = torch.zeros(c.scores.shape, device=cuda)
+            got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, **kw)
+            for b in range(B):
+                page, off = c.slots(b)
+                w = weights[b].t()[P:]
+                assert ((sc.cpu().double()[page[P:], :, off[P:]] - w).abs() <= (2 * rel + 2.0 ** -23 * (Hq // Hkv + 2)) * w).all()
+        else:
+            got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, seq_starts=st, max_q=max(n), **kw)
+        check(got, want, mag, F16, rel)
+        assert (buffer[size:] == 255).all()
