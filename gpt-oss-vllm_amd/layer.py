@@ -137,8 +137,8 @@ class GptOssDecodeLayer:
 
     weights: dict with ln1, ln2 [H]; wqkv [(Hq + 2 Hkv) D][H], bqkv; wo [H][Hq D], bo; sinks [Hq] or None;
     router_w [E][H], router_b [E] or None; w13_q, w13_absmax, w2_q, w2_absmax (tile order), b13 / b2 or None -- fp16
-    unless NF4.  Every intermediate lives in buffers sized for max_tokens, so a step allocates nothing and can be
-    captured in a HIP graph.
+    unless NF4.  Every intermediate lives in buffers sized for max_tokens, so a step allocates nothing (but for
+    the attention's workspace, where it needs a larger one than any step before) and can be captured in a HIP graph.
     """
 
     def __init__(self, weights, *, hidden: int, heads: int, kv_heads: int, head_dim: int, ffn: int, experts: int,
@@ -163,6 +163,18 @@ class GptOssDecodeLayer:
         self.moe_out = torch.empty((T, hidden), **f16)
         self.moe_ws = torch.empty(max(256, lib.moe_workspace_bytes(T, top_k, hidden, ffn, experts)), dtype=torch.uint8, device=dev)
         self.attn_ws = None
+        self._captured, self._outgrown = False, []
+
+    def _attn_workspace(self, need: int):
+        """The attention's workspace of at least `need` bytes.  One that a captured graph writes to on every replay is kept
+        when a later call (another form, a longer context) needs a larger one."""
+        if need and (self.attn_ws is None or self.attn_ws.numel() < need):
+            if self._captured:
+                self._outgrown.append(self.attn_ws)
+            self.attn_ws, self._captured = torch.empty(need, dtype=torch.uint8, device=self.q.device), False
+        if self.attn_ws is not None and torch.cuda.is_current_stream_capturing():
+            self._captured = True
+        return self.attn_ws
 
     def write_kv_only(self, x, positions, slots, kcache, vcache, cos, sin):
         """RMSNorm + q/k/v projection + rotary + cache write for tokens whose attention output is not needed
@@ -234,9 +246,7 @@ class GptOssDecodeLayer:
             need = lib.shared_prefix_attn_workspace_bytes(T, T, 1, self.Hq, self.Hkv, self.D, max_ctx, prefix_len)
         else:
             need = lib.paged_attn_workspace_bytes(T, self.Hq, self.D, max_ctx)
-        if need and (self.attn_ws is None or self.attn_ws.numel() < need):
-            self.attn_ws = torch.empty(need, dtype=torch.uint8, device=self.q.device)
-        attn_args = dict(max_ctx=max_ctx, scale=self.D ** -0.5, workspace=self.attn_ws, out=self.attn, sinks=w.get("sinks"), window=self.window)
+        attn_args = dict(max_ctx=max_ctx, scale=self.D ** -0.5, workspace=self._attn_workspace(need), out=self.attn, sinks=w.get("sinks"), window=self.window)
         if scores is not None:
             lib.paged_attn_decode_scored(self.q, kcache, vcache, scores, block_tables, ctx_lens, prefix_len=prefix_len, **attn_args)
         elif prefix_len:

@@ -291,3 +291,110 @@ def test_gpu_results_hold_for_every_workspace(case, scored, m355, cuda):
             got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, seq_starts=st, max_q=max(n), **kw)
         check(got, want, mag, F16, rel)
         assert (buffer[size:] == 255).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the decoder layer
+# ---------------------------------------------------------------------------------------------------------------------
+def test_layer_keeps_a_workspace_that_a_graph_was_captured_with(monkeypatch):
+    """A larger workspace replaces the layer's, but one that a captured graph writes to stays allocated; one that no graph
+    uses is let go."""
+    import weakref
+
+    from gpt_oss_vllm_amd import layer
+    lyr = layer.GptOssDecodeLayer.__new__(layer.GptOssDecodeLayer)
+
+    class Calls:
+        """Stands for the library: every call is a no-op that hands out what forward() asks of it."""
+        FLAG_SKIP_COMBINE = 1
+        used = None
+
+        def __getattr__(self, name):
+            if name.endswith("workspace_bytes"):
+                return lambda *a, **kw: self.need
+            if name in ("paged_attn_decode", "paged_attn_decode_scored", "shared_prefix_attn"):
+                return lambda *a, **kw: setattr(self, "used", kw["workspace"])
+            return lambda *a, **kw: None
+
+    lib = Calls()
+    t = torch.zeros((1, 64))
+    lyr.__dict__.update(dict.fromkeys("h1 resid qkv resid2 h2 ids wts moe_out moe_ws".split(), t), lib=lib, w=dict.fromkeys("ln1 wqkv wo ln2 router_w w13_q w13_absmax w2_q w2_absmax".split()),
+                        T=1, Hq=1, Hkv=1, D=64, FF=1, E=1, k=1, H=64, eps=1e-5, window=0, act_mode=0, q=t.view(1, 1, 64), attn=t.view(1, 1, 64))
+    lyr.attn_ws = None
+    lyr._captured, lyr._outgrown = False, []
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+
+    def step(need, **kw):
+        lib.need = need
+        lyr.forward(t, *[None] * 9, max_ctx=9, **kw)
+        assert lib.used is not None and lib.used.numel() >= need
+        return weakref.ref(lib.used), lib.used.data_ptr()
+
+    eager, _ = step(100)
+    capturing[0] = True
+    first, at = step(200, prefix_len=3)
+    capturing[0] = False
+    lib.used = None
+    assert eager() is None                                        # no graph uses it
+    second, _ = step(5000, scores=t)
+    lib.used = None
+    assert first() is not None and first().data_ptr() == at       # the graph goes on writing there
+    step(9000, scores=t)
+    lib.used = None
+    assert second() is None and first() is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["full", "sliding"])
+def test_gpu_layer_graphs_outlive_larger_steps(name, m355, cuda):
+    """A plain step, one behind a shared prefix and a scored one, captured one after the other with growing needs, eager steps
+    that need still more in between, other tensors allocated and filled: every replay gives the eager result and leaves
+    those tensors as they are."""
+    from gpt_oss_vllm_amd import layer
+    from test_layer_ops import _decoder_layer
+    B, bs, P, ctx = 3, 16, 96, 201
+    lyr, p = _decoder_layer(name, B)
+    Hkv, D = p["Hkv"], p["D"]
+    blocks = B * 320
+    g = torch.Generator().manual_seed(4)
+    bt = torch.randperm(blocks, generator=g).view(B, -1).to(torch.int32).to(cuda)          # 320 pages each: contexts of up to 5120
+    kc = torch.randn((blocks, bs, Hkv, D), generator=g).to(F16).to(cuda)
+    vc = torch.randn((blocks, bs, Hkv, D), generator=g).to(F16).to(cuda)
+    cos, sin = (t.to(cuda) for t in layer.rope_tables(8192))
+    x = torch.from_numpy(p["x"]).to(cuda)[:B].contiguous()
+    pos = torch.full((B,), ctx - 1, dtype=torch.int32, device=cuda)
+    slots = bt[:, (ctx - 1) // bs].long() * bs + (ctx - 1) % bs
+    lens = torch.full((B,), ctx, dtype=torch.int32, device=cuda)
+    scores = torch.zeros((blocks, Hkv, bs), device=cuda)
+    forms = [dict(max_ctx=600), dict(max_ctx=1500, prefix_len=P), dict(max_ctx=3000, prefix_len=P, scores=scores)]
+
+    def step(kw):
+        scores.zero_()
+        r, m = lyr.forward(x, None, pos, slots, bt, lens, kc, vc, cos, sin, **kw)
+        return r, m
+
+    def result(kw):
+        r, m = step(kw)
+        torch.cuda.synchronize()
+        return r.clone(), m.clone(), scores.clone()
+
+    graphs, wants = [], []
+    for kw in forms:
+        wants.append(result(kw))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(kw)
+        graphs.append(graph)
+    others = []
+    for turn in range(3):
+        result(dict(max_ctx=5120 - 16 * (2 - turn), prefix_len=P, scores=scores))            # needs more than any step before
+        others += [torch.full((n,), 7.0, device=cuda) for n in (1 << 10, 1 << 14, 1 << 16, 1 << 18, 1 << 20, 1 << 21) for _ in range(4)]
+        for graph, want in zip(graphs, wants):
+            lyr.resid2.zero_(), lyr.moe_out.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for got, exp in zip((lyr.resid2, lyr.moe_out, scores), want):
+                assert torch.equal(got, exp)
+        assert all((t == 7.0).all() for t in others)
