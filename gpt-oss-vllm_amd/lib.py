@@ -834,13 +834,17 @@ def shared_prefix_attn_workspace_bytes(T: int, B: int, max_q: int, Hq: int, Hkv:
 
 
 def shared_prefix_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, *,
-                       prefix_len: int, max_ctx: int, scale: float, seq_starts: Optional[torch.Tensor] = None, max_q: int = 1,
+                       prefix_len: int, max_ctx: int, scale: float, seq_starts: Optional[torch.Tensor] = None, max_q: Optional[int] = None,
                        sinks: Optional[torch.Tensor] = None, window: int = 0, workspace: Optional[torch.Tensor] = None,
                        out: Optional[torch.Tensor] = None):
     """Attention of new tokens q [T][Hq][D] (fp16 or bf16; tokens may be strided) over a paged cache whose first prefix_len
     tokens, read through row 0 of block_tables, all sequences share.  seq_starts int32 [B + 1] gives the sequences' tokens,
-    max_q the longest one's number; without it there is one token per sequence.  ctx_lens count the new tokens.
-    m355_shared_prefix_attn."""
+    max_q the longest one's number (tokens behind it are left out, so both go together); without them there is one token per
+    sequence.  ctx_lens count the new tokens.  m355_shared_prefix_attn."""
+    if max_q is None:
+        if seq_starts is not None:
+            raise ValueError("seq_starts needs max_q, the longest sequence's number of new tokens")
+        max_q = 1
     _one_device(("q", "kcache", "vcache", "block_tables", "ctx_lens", "seq_starts", "sinks", "workspace", "out"), q, kcache, vcache,
                 block_tables, ctx_lens, seq_starts, sinks, workspace, out)
     if q.dtype not in _DTYPE_CODES:

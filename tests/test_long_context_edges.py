@@ -294,6 +294,17 @@ def test_gpu_results_hold_for_every_workspace(case, scored, m355, cuda):
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------------------------------------------------
+def test_several_tokens_need_their_longest_number(m355):
+    """Without max_q a packed call would leave all tokens but the sequences' first ones unwritten."""
+    c = Cache(1, [20, 30], 2, 64, 16, F16)
+    q, st = torch.zeros((5, 8, 64), dtype=F16), torch.tensor([0, 2, 5], dtype=torch.int32)
+    with pytest.raises(ValueError, match="max_q"):
+        m355.shared_prefix_attn(q, c.k, c.v, c.tables, torch.tensor(c.ctx, dtype=torch.int32), prefix_len=0, max_ctx=32, scale=0.1, seq_starts=st)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
 def test_layer_keeps_a_workspace_that_a_graph_was_captured_with(monkeypatch):
