@@ -79,10 +79,11 @@ def validate_eviction(block_tables: torch.Tensor, ctx_lens: torch.Tensor, dst_ta
     nblocks, block_size = kcache.shape[0], kcache.shape[1]
     src, dst = block_tables.detach().cpu(), dst_tables.detach().cpu()
     first, seen = prefix_len // block_size, set()
-    read = set()
+    # the shared pages (row 0's leading entries; the other rows' may hold anything) and every sequence's own ones
+    read = set(src[0, :first].tolist()) if src.shape[0] else set()
     for b, ctx in enumerate(ctx_lens.detach().cpu().tolist()):
-        read.update(src[b if ctx > prefix_len else 0, :(ctx + block_size - 1) // block_size].tolist())
-    read.update(src[0, :first].tolist())
+        if ctx > prefix_len:
+            read.update(src[b, first:(ctx + block_size - 1) // block_size].tolist())
     for b, ctx in enumerate(ctx_lens.detach().cpu().tolist()):
         end = prefix_len + min(max(ctx - prefix_len, 0), keep)
         need = (end + block_size - 1) // block_size

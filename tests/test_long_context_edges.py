@@ -304,6 +304,25 @@ def test_several_tokens_need_their_longest_number(m355):
         m355.shared_prefix_attn(q, c.k, c.v, c.tables, torch.tensor(c.ctx, dtype=torch.int32), prefix_len=0, max_ctx=32, scale=0.1, seq_starts=st)
 
 
+def test_validate_eviction_reads_shared_pages_through_row_0():
+    """Leading entries of the other rows may be padding or stale: a destination page of the same number is free.  Pages that
+    are shared, or hold a sequence's own tokens, or are handed out twice, are not."""
+    from gpt_oss_vllm_amd.layer import validate_eviction
+    kc = torch.zeros((12, 16, 1, 64), dtype=F16)
+    src = torch.tensor([[7, 8, 3, 4], [0, 5, 1, 2], [9, 9, 9, 9]], dtype=torch.int32)     # prefix: pages 7 and 8
+    lens = torch.tensor([60, 64, 20], dtype=torch.int32)                                   # the third ends inside the prefix
+    dst = torch.tensor([[7, 8, 0], [7, 8, 5], [7, 8, 9]], dtype=torch.int32)
+    validate_eviction(src, lens, dst, kc, keep=10, prefix_len=32)
+    for row, page, why in ((0, 7, "in use"), (0, 8, "in use"), (1, 3, "in use"), (0, 2, "in use"), (1, 0, "in use"), (0, 12, "outside"), (1, -1, "outside")):
+        bad = dst.clone()
+        bad[row, 2] = page
+        with pytest.raises(ValueError, match=why):
+            validate_eviction(src, lens, bad, kc, keep=10, prefix_len=32)
+    with pytest.raises(ValueError, match="holds 3"):
+        validate_eviction(src, lens, dst, kc, keep=17, prefix_len=32)
+    validate_eviction(src[:0], lens[:0], dst[:0], kc, keep=10, prefix_len=32)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
