@@ -104,6 +104,9 @@ def evict_tokens(caches, scores, block_tables: torch.Tensor, ctx_lens: torch.Ten
     tables and lengths (returned) serve them all; `recent` of at least a sliding window leaves windowed layers unharmed.
     Rotary positions go on counting from the old lengths: keys were rotated when they were written."""
     from . import lib
+    caches, scores = list(caches), list(scores)
+    if len(caches) != len(scores):
+        raise ValueError(f"{len(caches)} layers' caches, {len(scores)} layers' scores: the layers left out would not fit the new lengths")
     for (kc, vc), sc in zip(caches, scores):
         _, new_lens = lib.kv_evict(kc, vc, sc, block_tables, ctx_lens, dst_tables, keep=keep, recent=recent, max_ctx=max_ctx,
                                    prefix_len=prefix_len, new_lens=new_lens)

@@ -323,6 +323,19 @@ def test_validate_eviction_reads_shared_pages_through_row_0():
     validate_eviction(src[:0], lens[:0], dst[:0], kc, keep=10, prefix_len=32)
 
 
+def test_evict_tokens_takes_every_layer_or_none(monkeypatch, m355):
+    """Caches without scores of their own would keep their old rows under the new lengths."""
+    from gpt_oss_vllm_amd import layer
+    seen = []
+    monkeypatch.setattr(m355, "kv_evict", lambda kc, vc, sc, *a, **kw: seen.append((kc, sc)) or (None, "lens"))
+    args = dict(keep=4, recent=1, max_ctx=32)
+    for caches, scores in (([(1, 1), (2, 2)], [3]), ([(1, 1)], [3, 4]), ([(1, 1)], [])):
+        with pytest.raises(ValueError, match="layers"):
+            layer.evict_tokens(caches, scores, None, None, None, **args)
+    assert not seen
+    assert layer.evict_tokens(iter([(1, 1), (2, 2)]), iter([3, 4]), None, None, None, **args) == "lens" and seen == [(1, 3), (2, 4)]
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
