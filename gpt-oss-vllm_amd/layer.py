@@ -198,6 +198,10 @@ class GptOssDecodeLayer:
         the first prefix_len tokens are shared by all sequences (m355_shared_prefix_attn), and every token needs a slot.
         Buffers are allocated per call (prompt sizes vary).  Returns (residual stream after attention, expert output), as
         forward does."""
+        if block_tables is None and (ctx_lens is not None or max_ctx or prefix_len):
+            raise ValueError("ctx_lens, max_ctx and prefix_len belong to prompts that continue a cache: block_tables is missing")
+        if block_tables is not None and (ctx_lens is None or max_ctx <= 0):
+            raise ValueError("prompts that continue a cache need ctx_lens and max_ctx")
         lib, w = self.lib, self.w
         T, dev = resid_in.shape[0], resid_in.device
         resid = torch.empty_like(resid_in)

@@ -336,6 +336,17 @@ def test_evict_tokens_takes_every_layer_or_none(monkeypatch, m355):
     assert layer.evict_tokens(iter([(1, 1), (2, 2)]), iter([3, 4]), None, None, None, **args) == "lens" and seen == [(1, 3), (2, 4)]
 
 
+def test_prefill_refuses_half_a_continuation():
+    """Prompts that continue a cache name its tables, lengths and bound; without tables the rest would be ignored and the
+    prompt attend to itself alone."""
+    from gpt_oss_vllm_amd import layer
+    lyr = layer.GptOssDecodeLayer.__new__(layer.GptOssDecodeLayer)
+    t = torch.zeros((1, 64))
+    for kw in (dict(prefix_len=8), dict(max_ctx=9), dict(ctx_lens=t), dict(block_tables=t), dict(block_tables=t, ctx_lens=t), dict(block_tables=t, max_ctx=8)):
+        with pytest.raises(ValueError, match="continue a cache"):
+            lyr.prefill(t, None, None, None, None, 1, None, None, None, None, **kw)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
