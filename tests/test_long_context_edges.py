@@ -347,6 +347,21 @@ def test_prefill_refuses_half_a_continuation():
             lyr.prefill(t, None, None, None, None, 1, None, None, None, None, **kw)
 
 
+def _evict_answer(m355, **kw):
+    p = 0x10000
+    a = dict(kc=p, vc=p, scores=p, tables=p, ctx=p * 2, dst=p, B=4, Hkv=2, row_bytes=128, num_blocks=9, block_size=16, max_blocks=4,
+             max_dst=3, stride=16 * 2 * 128, max_ctx=64, prefix=16, keep=32, recent=4, kept=p, new_lens=p * 3)
+    a.update(kw)
+    return m355.load().m355_kv_evict(*a.values(), None)
+
+
+def test_kv_evict_refuses_sizes_that_its_counters_do_not_hold(m355):
+    """A list of nearly 2^31 entries (its loops would step past the type's end), rows of more than 2^20 bytes (32 of them are
+    counted in 16-byte pieces); refused before anything is launched."""
+    for kw in (dict(keep=(1 << 31) - 1), dict(keep=(1 << 30) + 1), dict(row_bytes=1 << 30, stride=16 * 2 << 30), dict(row_bytes=(1 << 20) + 16, stride=1 << 30)):
+        assert _evict_answer(m355, **kw) == -2, kw
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
