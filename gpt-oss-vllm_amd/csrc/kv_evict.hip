@@ -532,7 +532,7 @@ extern "C" int m355_kv_evict(void* kcache, void* vcache, float* scores, const in
     if (block_stride_bytes < (int64_t)block_size * Hkv * row_bytes || block_stride_bytes % 16)
         return fail(-2, "m355_kv_evict: a page stride of %lld bytes (need at least block_size*Hkv*row_bytes, a multiple of 16)", (long long)block_stride_bytes);
     if (!aligned(kcache, 16) || !aligned(vcache, 16)) return fail(-3, "m355_kv_evict: caches must be 16-byte aligned");
-    if (new_lens == ctx_lens) return fail(-2, "m355_kv_evict: new_lens must not be ctx_lens");
+    if (new_lens < ctx_lens + B && ctx_lens < new_lens + B) return fail(-2, "m355_kv_evict: new_lens must not overlap ctx_lens");
     const int64_t chunks = (most + EV_ROWS - 1) / EV_ROWS;
     if ((int64_t)B * Hkv * (chunks + 1) >= (1ll << 30)) return fail(-2, "m355_kv_evict: unsupported size B=%d Hkv=%d keep=%d", B, Hkv, keep);
     uint32_t page_mul;

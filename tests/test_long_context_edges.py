@@ -362,6 +362,14 @@ def test_kv_evict_refuses_sizes_that_its_counters_do_not_hold(m355):
         assert _evict_answer(m355, **kw) == -2, kw
 
 
+def test_kv_evict_refuses_new_lengths_over_the_old_ones(m355):
+    """Every head of a sequence reads the old length while the first one writes the new: they share no entry (B is 4)."""
+    for entries in (-3, -1, 0, 1, 3):
+        assert _evict_answer(m355, new_lens=0x20000 + 4 * entries) == -2, entries
+        assert b"new_lens" in m355.load().m355_last_error()
+    assert _evict_answer(m355, new_lens=0x20000 + 16, B=0) == 0
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the decoder layer
 # ---------------------------------------------------------------------------------------------------------------------
