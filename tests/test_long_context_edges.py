@@ -475,3 +475,84 @@ def test_gpu_layer_graphs_outlive_larger_steps(name, m355, cuda):
             for got, exp in zip((lyr.resid2, lyr.moe_out, scores), want):
                 assert torch.equal(got, exp)
         assert all((t == 7.0).all() for t in others)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# forms of the kernels that only larger calls take
+# ---------------------------------------------------------------------------------------------------------------------
+def _scored_check(m355, cuda, c, q, sk, scale, window, max_ctx=None):
+    B, P = len(c.ctx), c.prefix
+    want, mag, weights = oracle(c, q, [1] * B, scale, sk, window)
+    kc, vc, bt, cl = c.device(cuda)
+    sc = c.scores.to(cuda)
+    rel = score_err(c, q, scale)
+    got = m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, max_ctx=max_ctx or max(c.ctx), scale=scale, prefix_len=P,
+                                        sinks=None if sk is None else sk.to(cuda), window=window)
+    check(got, want, mag, c.dtype, rel)
+    exp, tol = c.scores.double().clone(), torch.zeros(c.scores.shape, dtype=torch.float64)
+    for b in range(B):
+        page, off = c.slots(b)
+        w = weights[b].t()[P:]
+        exp[page[P:], :, off[P:]] += w
+        # G weights of relative error rel and their sum, then a rounded addition
+        tol[page[P:], :, off[P:]] = (2 * rel + 2.0 ** -23 * (q.shape[1] // c.Hkv)) * w
+    tol += 2.0 ** -23 * exp * (tol > 0)
+    assert ((sc.cpu().double() - exp).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("window", [0, 900])
+def test_gpu_scored_batch_of_wide_heads_behind_a_prefix(dtype, window, m355, cuda):
+    """128 rows per workgroup over the prefix, heads of 128, beside scored own tokens."""
+    own = [1 + 7 * b % 50 for b in range(40)]
+    c = Cache(21, [2500 + o for o in own], 4, 128, 16, dtype, prefix=2500, poison=True, window=window)
+    q, sk = _inputs(c, 40, 32, 8, True)
+    _scored_check(m355, cuda, c, q, sk, 128 ** -0.5, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gpu_scored_many_sequences(dtype, m355, cuda):
+    """More than 16384 rows: several rows per wave in the joining, and the weights in the same launch."""
+    own = [1 + 13 * b % 305 for b in range(260)]
+    c = Cache(22, [800 + o for o in own], 8, 64, 16, dtype, prefix=800, poison=True)
+    q, sk = _inputs(c, 260, 64, 9, True)
+    _scored_check(m355, cuda, c, q, sk, 0.125, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, D, dtype", [((72, 1), 64, F16), ((130, 1), 64, BF16), ((72, 1), 128, BF16), ((130, 1), 128, F16), ((144, 2), 64, F16)])
+@pytest.mark.parametrize("P, own, block, window", [(0, [400, 9, 65], 16, 0), (300, [1800, 1, 700], 20, 0), (4050, [3, 50, 1], 64, 0), (300, [1800, 1, 700], 16, 500)])
+def test_gpu_scored_more_than_64_heads_on_one_kv_head(heads, D, dtype, P, own, block, window, m355, cuda):
+    """The weights of such a group are added up 64 heads at a time."""
+    c = Cache(23, [P + o for o in own], heads[1], D, block, dtype, prefix=P, poison=True, window=window)
+    q, sk = _inputs(c, len(own), heads[0], 10, True)
+    _scored_check(m355, cuda, c, q, sk, D ** -0.5, window, max_ctx=c.tables.shape[1] * block)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gpu_many_sequences_of_wide_heads_on_a_long_prefix(dtype, m355, cuda):
+    """More than 16384 rows of 128 columns: two rows per wave in the joining."""
+    own = [1 + b % 5 for b in range(600)]
+    c = Cache(24, [1500 + o for o in own], 8, 128, 16, dtype, prefix=1500, poison=True)
+    q, sk = _inputs(c, 600, 32, 11, True)
+    want, mag, _ = oracle(c, q, [1] * 600, 128 ** -0.5, sk)
+    kc, vc, bt, cl = c.device(cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=1500, max_ctx=max(c.ctx), scale=128 ** -0.5, sinks=sk.to(cuda))
+    check(got, want, mag, dtype, score_err(c, q, 128 ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gpu_prompts_of_many_rows_on_a_long_prefix(dtype, m355, cuda):
+    """256 rows per workgroup over the prefix, 128 over the prompts' own tokens."""
+    n, P = [300, 260], 4101
+    c = Cache(25, [P + k for k in n], 8, 64, 16, dtype, prefix=P, poison=True, n=n)
+    q, sk = _inputs(c, sum(n), 64, 12, True)
+    want, mag, _ = oracle(c, q, n, 0.125, sk)
+    kc, vc, bt, cl = c.device(cuda)
+    st = torch.tensor([0, 300, 560], dtype=torch.int32, device=cuda)
+    got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125, seq_starts=st, max_q=300, sinks=sk.to(cuda))
+    check(got, want, mag, dtype, score_err(c, q, 0.125))
