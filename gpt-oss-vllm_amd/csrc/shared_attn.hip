@@ -612,41 +612,70 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                 *reinterpret_cast<float4_t*>(at + qi * D * 4 + (((8 * dt + 2 * i4 + hh) ^ (qi & 15)) << 4)) =
                     float4_t{acc[dt][4 * i4], acc[dt][4 * i4 + 1], acc[dt][4 * i4 + 2], acc[dt][4 * i4 + 3]};
     };
-    // An output may be NaN only because an infinite value met a probability that rounds to 0: then the values of that column
-    // that the row sees are looked through once more (tiles that are seen in part count them in the walk).
+    // An output may be NaN only because an infinite value met a probability that rounds to 0: then the values of its column
+    // that the row sees are looked through once more (tiles that are seen in part count them in the walk).  What all the
+    // wave's rows see is looked through once, several keys at a time, the rest row by row: 65536 keys take some ms, and only
+    // where an output is NaN.
     auto settle = [&](unsigned char* at, const f32x16_t(&acc)[DT], float l, int row_pos, int row_lo) {
         float z[4] = {0.f, 0.f, 0.f, 0.f};   // (0 times an infinity or NaN: one instruction per value)
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) z[i & 3] = __builtin_fmaf(acc[dt][i], 0.f, z[i & 3]);
-        if (!__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f)) return;
+        if (__builtin_expect(!__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f), 1)) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int c = lane % CH;
+        // bit e (e + 4): column 4 c + e holds a value that is +inf or NaN (-inf or NaN), keys from, from + by, .. upto
+        auto look = [&](int from, int upto, int by) {
+            constexpr int AT_ONCE = 4;
+            uint32_t found = 0;
+            for (int key0 = from; key0 <= upto && found != 0xffu; key0 += AT_ONCE * by) {
+                u32x2_t raw[AT_ONCE];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) {
+                    const int key = min(key0 + u * by, upto), page = page_of(a, key);
+                    const int blk = min(max(key < folded ? a.tables[page] : table[page], 0), a.num_blocks - 1);
+                    const int64_t off = blk * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D + 4 * c;
+                    raw[u] = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const E*>(a.vc) + off);
+                }
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) {
+                    u32x4_t clean, p, m;
+                    if (!split_nonfinite<E>(u32x4_t{raw[u][0], raw[u][1], 0u, 0u}, clean, p, m)) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        found |= (p[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 1u << e : 0u;
+                        found |= (m[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 16u << e : 0u;
+                    }
+                }
+            }
+            return found;
+        };
+        const int all_first = max(kfloor, lo_max), all_last = min(kend - 1, pos_min);
+        int seen = (int)look(all_first + lane / CH, all_last, 64 / CH);
+#pragma unroll
+        for (int st = CH; st < 64; st *= 2) seen |= __shfl_xor(seen, st, 64);
 #pragma unroll 1
         for (int i = 0; i < 32 * CH / 64; i++) {
-            const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+            const int r = i * (64 / CH) + lane / CH;
             const int first = max(kfloor, __shfl(row_lo, r, 64)), last = min(kend - 1, __shfl(row_pos, r, 64));
             const float lr = __shfl(l, r, 64);
             float4_t* to = reinterpret_cast<float4_t*>(at + r * D * 4 + ((c ^ (r & 15)) << 4));
             float4_t v = *to;
-            uint32_t asked = 0, plus = 0, minus = 0;   // bit e: column 4 c + e
+            bool asked[4], any = false;
 #pragma unroll
-            for (int e = 0; e < 4; e++) asked |= lr == lr && v[e] != v[e] ? 1u << e : 0u;   // (l is NaN where a score is)
-            for (int key = first; key <= last && (plus & minus & asked) != asked; key++) {
-                const int page = page_of(a, key), blk = min(max(key < folded ? a.tables[page] : table[page], 0), a.num_blocks - 1);
-                const int64_t off = blk * a.block_stride + ((int64_t)(key - page * a.block_size) * a.Hkv + hk) * D + 4 * c;
-                const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const E*>(a.vc) + off);
-                u32x4_t clean, p, m;
-                if (split_nonfinite<E>(u32x4_t{raw[0], raw[1], 0u, 0u}, clean, p, m))
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        plus |= (p[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 1u << e : 0u;
-                        minus |= (m[e / 2] >> 16 * (e & 1) & 0xffffu) != 0 ? 1u << e : 0u;
-                    }
+            for (int e = 0; e < 4; e++) any |= asked[e] = lr == lr && v[e] != v[e];   // (l is NaN where a score is)
+            if (!any) continue;
+            uint32_t found = (uint32_t)seen;
+            if (all_first > all_last) {
+                found |= look(first, last, 1);
+            } else {
+                found |= look(first, all_first - 1, 1);
+                found |= look(all_last + 1, last, 1);
             }
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (asked & (plus ^ minus) & 1u << e) v[e] = plus >> e & 1 ? INFINITY : -INFINITY;
+                if (asked[e] && (found >> e & 1) != (found >> (e + 4) & 1)) v[e] = found >> e & 1 ? INFINITY : -INFINITY;
             *to = v;
         }
     };

@@ -556,3 +556,31 @@ def test_gpu_prompts_of_many_rows_on_a_long_prefix(dtype, m355, cuda):
     st = torch.tensor([0, 300, 560], dtype=torch.int32, device=cuda)
     got = m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, prefix_len=P, max_ctx=max(c.ctx), scale=0.125, seq_starts=st, max_q=300, sinks=sk.to(cuda))
     check(got, want, mag, dtype, score_err(c, q, 0.125))
+
+
+@pytest.mark.gpu
+def test_gpu_infinite_values_in_a_long_context(m355, cuda):
+    """Values that are infinite all along a context of 60000 tokens, far below the key that dominates: looking for them takes
+    milliseconds, not a walk per row."""
+    L = 60000
+    c = Cache(27, [L, 40], 2, 64, 64, F16)
+    c.k[..., 0] = 0
+    page, off = c.slots(0)
+    c.k[page[L - 1], off[L - 1], :, 0] = 60
+    c.v[page[:-1], off[:-1], 0, 5] = float("inf")
+    c.v[page[::2], off[::2], 1, 9], c.v[page[1::2], off[1::2], 1, 9] = float("inf"), float("-inf")
+    q = torch.zeros((2, 64, 64), dtype=F16)
+    q[..., 0] = 8
+    kc, vc, bt, cl = c.device(cuda)
+    args = (q.to(cuda), kc, vc, bt, cl)
+    for run in range(2):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        got = m355.shared_prefix_attn(*args, prefix_len=0, max_ctx=L, scale=0.125, workspace=torch.empty(256, dtype=torch.uint8, device=cuda))
+        end.record()
+        torch.cuda.synchronize()
+    assert start.elapsed_time(end) < 500.0
+    got = got.cpu()
+    assert (got[0, :32, 5] == float("inf")).all() and got[0, 32:, 9].isnan().all()
+    got[0, :32, 5] = got[0, 32:, 9] = 0
+    assert got.isfinite().all()
