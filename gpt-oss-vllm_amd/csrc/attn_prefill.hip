@@ -33,19 +33,6 @@ typedef __attribute__((address_space(3))) short4_t ap_lds_s4_t;
 typedef __attribute__((address_space(3))) void ap_lds_void_t;
 typedef const __attribute__((address_space(1))) void ap_glb_void_t;
 
-// Combine a value with the one lane ^ 32 holds: one v_permlane32_swap (the upper half of the first operand trades places
-// with the lower half of the second) leaves both halves' values on every lane, no LDS round trip.
-__device__ __forceinline__ float cross_half_max(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
-}
-__device__ __forceinline__ float cross_half_sum(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
-}
-
 __global__ __launch_bounds__(AP_THREADS) void attn_prefill_kernel(
     const half_t* __restrict__ q, const half_t* __restrict__ k, const half_t* __restrict__ v,
     const int32_t* __restrict__ seq_starts, int Hq, int64_t q_stride, int64_t kv_stride, int64_t o_stride, float scale,

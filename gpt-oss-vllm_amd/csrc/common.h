@@ -74,6 +74,19 @@ inline void divide_by(int d, uint32_t& mul, int& shift) {
 }
 
 // ---- device helpers ----
+// Combine a value with the one lane ^ 32 holds: one v_permlane32_swap (the upper half of the first operand trades places
+// with the lower half of the second) leaves both halves' values on every lane, no LDS round trip.
+__device__ __forceinline__ float cross_half_max(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+}
+__device__ __forceinline__ float cross_half_sum(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
+}
+
 // Reinterpret a dword as two fp16.  Always go through this by-value helper: __builtin_bit_cast applied
 // directly to an indexed vector element (v[j] with an unrolled loop index) was seen to read element 0
 // for every j with hipcc 7.2.

@@ -101,17 +101,6 @@ __device__ __forceinline__ int window_lo(const SharedAttnArgs& a, int pos) {
     return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
 }
 
-// The larger of this lane's value and the one lane ^ 32 holds: one v_permlane32_swap, no LDS round trip.
-__device__ __forceinline__ float half_max(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto sw = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
-}
 // Wave-wide minimum with DPP only (lanes that a step leaves out combine with themselves).
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ int dpp_min(int v) { return min(v, __builtin_amdgcn_update_dpp(v, v, CTRL, ROW_MASK, 0xf, false)); }
@@ -515,7 +504,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
                 float mx = fmaxf(fmaxf(x[q][0], x[q][1]), x[q][2]);
 #pragma unroll
                 for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, x[q][i]), x[q][i + 1]);
-                mx = fmaxf(half_max(fmaxf(mx, x[q][15])) * a.scale2 - LIFT, m_run[q]);
+                mx = fmaxf(cross_half_max(fmaxf(mx, x[q][15])) * a.scale2 - LIFT, m_run[q]);
                 const float alpha = __builtin_amdgcn_exp2f(m_run[q] - mx);   // (0 for the first key)
                 m_run[q] = mx;
                 l_run[q] *= alpha;
@@ -687,7 +676,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
 #pragma unroll
         for (int q = 0; q < QT; q++) {
             put(at, o[q]);
-            const float l = half_sum(l_run[q]);
+            const float l = cross_half_sum(l_run[q]);
             settle(at, o[q], l, pos[q], lo[q]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const int first = row0 + 32 * (wave * QT + q), c = lane % CH;
@@ -722,7 +711,7 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         static_assert(QT == 1 && 32 * D * 4 <= W::STAGE);
         __shared__ float wm[SA_WAVES][32], wl[SA_WAVES][32];
         put(tiles, o[0]);   // (each wave in place of its own tile)
-        const float lsum = half_sum(l_run[0]);
+        const float lsum = cross_half_sum(l_run[0]);
         settle(tiles, o[0], lsum, pos[0], lo[0]);
         if (hh == 0) {
             wm[wave][qi] = m_run[0];
