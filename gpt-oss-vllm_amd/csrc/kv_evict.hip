@@ -17,9 +17,10 @@ namespace m355 {
 
 constexpr int EV_THREADS = 256;
 // Up to so many bytes of K per head, the selection's workgroup copies the kept rows itself, without a second launch.  Measured,
-// one launch / two, us: rows of 128 bytes, 128 of 300 tokens, 16 heads 8.4 / 10.1; of 1000 tokens, 256 heads, 128 rows 11.7 /
-// 13.4, 512 rows 20.2 / 21.7; 16 heads, 512 rows 12.3 / 10.8; of 9000 tokens, 32 heads, 512 rows 18.8 / 19.0, 1024 rows 24.1 /
-// 19.7.  (And the second launch is 2.5 us of the host's time.)
+// kernels in one launch / two, us: rows of 128 bytes, 128 of 300 tokens, 16 heads 8.4 / 10.1; of 1000 tokens, 256 heads, 128 rows
+// 11.7 / 13.4, 512 rows 20.2 / 21.7; 16 heads, 512 rows 12.3 / 10.8; of 9000 tokens, 32 heads, 512 rows 18.8 / 19.0, 1024 rows
+// 24.1 / 19.7.  At the limit few heads lose 1.5 us on the GPU, less than the 2.5 us of the host's time that the second launch
+// costs (which a captured graph does not pay); many heads still gain.  The rule does not look at their number.
 constexpr int64_t EV_ONE_LAUNCH = 65536;
 
 struct EvictArgs {

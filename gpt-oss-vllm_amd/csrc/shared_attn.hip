@@ -18,9 +18,15 @@
 // What bounds it.  Own tokens: memory (32 sequences of 2500 tokens, 8 KV heads of 64: 164 MB in 35 us, 4.7 TB/s; a plain copy
 // of the card: 5.2).  A walk over a prefix: the chain of one wave per SIMD, products, exponentials and LDS reads behind one
 // another (1.0 us per 64 keys of 128 rows, D 64, where the matrix cores need 0.25), so that two workgroups per CU get 1.6 times
-// as much done; many rows: exponentials beside the products (6 prompts of 150 to 420 tokens behind 8192, 226 GFLOP: 322 us, 0.70
-// PFLOP/s of the 1.2 that a large product reaches).  Tried without gain: 64 keys at a time, a K tile's fragments read a tile
-// ahead, four or five tiles in LDS instead of three.  Few tokens: launches (7 us for one, 10 for the ranges and their joining).
+// as much done; matrix cores busy for 13 % of the busy CUs' cycles, vector instructions 40 %, waves waiting half of the time (32
+// tokens on 8192).  Many rows: vector instructions (about 90 per 32 keys and 32 rows, 16 of them exponentials; 59 % of the busy
+// cycles) and products (8; 34 %) almost one after the other, with two waves per SIMD (6 prompts of 150 to 420 tokens behind 8192,
+// 226 GFLOP: 317 us, 0.71 PFLOP/s of the 1.2 that a large product reaches).  Tried without gain: 64 keys at a time, a K tile's
+// fragments read a tile ahead, four or five tiles in LDS instead of three.  Few tokens: launches (7 us for one, 10 for the ranges
+// and their joining).
+// Registers: the walks over prefix and own tokens, their two loops and both endings are one kernel.  Heads of 128 use all 256
+// vector registers that two waves per SIMD leave and spill 5 to 14 more, the 256-row form 3; every form keeps 48 to 124
+// scalar registers in vector lanes.  What that costs has not been measured apart.
 #include "common.h"
 
 #include <algorithm>
