@@ -584,3 +584,45 @@ def test_gpu_infinite_values_in_a_long_context(m355, cuda):
     assert (got[0, :32, 5] == float("inf")).all() and got[0, 32:, 9].isnan().all()
     got[0, :32, 5] = got[0, 32:, 9] = 0
     assert got.isfinite().all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a cache of many gigabytes
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits(m355, cuda):
+    """Pages 2^30 elements apart, K and V of a page in one allocation: element offsets reach 2^32 and more."""
+    P, keep = 40, 33
+    c = Cache(26, [P + 30, P + 50], 2, 64, 32, F16, prefix=P, dst=0, spare=4)
+    used = sorted(set(c.tables[0, :3].tolist() + c.tables[1, 1:3].tolist()))
+    free = [p for p in range(c.n) if p not in used][:3]
+    stride = 1 << 30
+    big = torch.empty((c.n - 1) * stride + (1 << 20), dtype=F16, device=cuda)
+    shape, strides = tuple(c.k.shape), (stride, 2 * 64, 64, 1)
+    kc, vc = big.as_strided(shape, strides), big.as_strided(shape, strides, 1 << 19)
+    kc.copy_(c.k), vc.copy_(c.v)
+    assert (c.n - 1) * stride >= 1 << 32
+    q, sk = _inputs(c, 2, 16, 13, True)
+    want, mag, weights = oracle(c, q, [1, 1], 0.125, sk)
+    _, _, bt, cl = c.device(cuda)
+    sc = c.scores.to(cuda)
+    rel = score_err(c, q, 0.125)
+    kw = dict(prefix_len=P, max_ctx=P + 50, scale=0.125, sinks=sk.to(cuda))
+    check(m355.shared_prefix_attn(q.to(cuda), kc, vc, bt, cl, **kw), want, mag, F16, rel)
+    check(m355.paged_attn_decode_scored(q.to(cuda), kc, vc, sc, bt, cl, **kw), want, mag, F16, rel)
+    # the second sequence's tokens behind the first page, to free pages at the far end
+    dst = torch.tensor([[c.tables[0, 0], free[0], free[1]], [c.tables[0, 0], free[2], free[0]]], dtype=torch.int32)[1:]
+    lens = cl[1:].contiguous()
+    scores = sc.clone()
+    kept, new = m355.kv_evict(kc, vc, scores, bt[1:].contiguous(), lens, dst.to(cuda), keep=keep, recent=4, prefix_len=32, max_ctx=P + 50)
+    assert new.tolist() == [32 + keep]
+    for h in range(2):
+        src = kept[0, h].cpu().long()
+        page, off = c.tables[1].long()[src // 32], src % 32
+        to = torch.arange(32, 32 + keep)
+        tp, tf = dst[0].long()[to // 32], to % 32
+        for cache, first in ((kc, c.k), (vc, c.v)):
+            assert torch.equal(cache.cpu()[tp, tf, h], first[page, off, h])
+        own = sc.cpu()[c.tables[1].long()[torch.arange(32, P + 50) // 32], h, torch.arange(32, P + 50) % 32]
+        best = torch.argsort(own[:-4], descending=True, stable=True)[:keep - 4].sort().values + 32
+        assert torch.equal(src, torch.cat([best, torch.arange(P + 46, P + 50)]))
