@@ -518,8 +518,8 @@ extern "C" int m355_kv_evict(void* kcache, void* vcache, float* scores, const in
     if (!kcache || !vcache || !scores || !block_tables || !ctx_lens || !dst_tables || !kept || !new_lens)
         return fail(-1, "m355_kv_evict: null pointer");
     // (keep: the loops over a list step past it; row_bytes: EV_ROWS rows' pieces are counted in 32 bits)
-    if (B < 0 || Hkv <= 0 || row_bytes <= 0 || row_bytes % 16 || row_bytes > (1 << 20) || keep > (1 << 30) || num_blocks <= 0 || block_size <= 0 || max_blocks <= 0 || max_dst_blocks <= 0 ||
-        max_ctx <= 0 || max_ctx > (1 << 30) || prefix_len < 0 || keep <= 0 || recent < 0 || recent > keep)
+    if (B < 0 || Hkv <= 0 || row_bytes <= 0 || row_bytes % 16 || row_bytes > (1 << 20) || num_blocks <= 0 || block_size <= 0 || max_blocks <= 0 ||
+        max_dst_blocks <= 0 || keep > (1 << 30) || max_ctx <= 0 || max_ctx > (1 << 30) || prefix_len < 0 || keep <= 0 || recent < 0 || recent > keep)
         return fail(-2, "m355_kv_evict: unsupported shape B=%d Hkv=%d row_bytes=%d num_blocks=%d block_size=%d max_blocks=%d max_dst_blocks=%d "
                         "max_ctx=%d prefix_len=%d keep=%d recent=%d (need row_bytes %% 16 == 0, at most 2^20, 0 < keep <= 2^30, 0 <= recent <= keep)",
                     B, Hkv, row_bytes, num_blocks, block_size, max_blocks, max_dst_blocks, max_ctx, prefix_len, keep, recent);

@@ -474,13 +474,13 @@ __device__ __forceinline__ void attend(const SharedAttnArgs& a, unsigned char* s
         // The exponents' reference follows the running maximum lazily: probabilities are formed against the old one, and only
         // if one of them exceeds LIMIT (seen on the packed 16-bit values, whose order is that of whole numbers) do the maximum,
         // the rescaling and the probabilities take another turn: a few times per row instead of a maximum per tile.  The
-        // denominator carries the same factor.  fp16 ends at 2^-24 below and 65504 above, so its
-        // reference is put 2^LIFT below the maximum: a row's largest probability is held as 2^9 to 2^16, and one that falls
-        // out of the normal range is off by at most 2^-34 of the largest (2^-25 with the maximum itself as the reference, which
-        // lost thousands of keys 18 nats below one that dominates).  A higher lift leaves less room before the next turn: 2^9
-        // costs nothing, 2^10 1 %, 2^11 4 % (32 tokens on 8192, drafted tokens, prompts).  bf16 has the exponents of fp32, its
-        // values too: there the reference lies above the maximum, so that no probability exceeds 2^-16 and 65536 of them times
-        // the largest finite value still add up to a finite sum.
+        // denominator carries the same factor.  fp16 ends at 2^-24 below and 65504 above, so its reference is put 2^LIFT below the
+        // maximum: a row's largest probability is held as 2^9 to 2^16, and one that falls out of the normal range is off by at
+        // most 2^-34 of the largest (2^-25 with the maximum itself as the reference, which lost thousands of keys 18 nats below
+        // one that dominates).  A higher lift leaves less room before the next turn: 2^9 costs nothing, 2^10 1 %, 2^11 4 % (32
+        // tokens on 8192, drafted tokens, prompts).  bf16 has the exponents of fp32, its values too: there the reference lies
+        // above the maximum, so that no probability exceeds 2^-16 and 65536 of them times the largest finite value still add up
+        // to a finite sum.
         uint32_t pb[QT][8];
         float sum[QT];
         auto exponentials = [&] {

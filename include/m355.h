@@ -417,9 +417,9 @@ M355_API size_t m355_paged_attn_decode_scored_workspace_bytes(int B, int Hq, int
  *   behind prefix_len (pages of the prefix stay shared and are not touched; prefix_len is a multiple of block_size).  The
  *   source pages stay as they are, for the caller to release.  kept [B][Hkv][keep] receives the kept positions in order
  *   (-1 behind them), new_lens [B] (no entry of ctx_lens) the new context length (prefix_len + kept tokens; a sequence that
- *   ends inside the prefix keeps its length).  Scores of the rows behind the last kept token in its page become 0.  row_bytes: bytes of one token's
- *   row of one KV head (D * element size, a multiple of 16, at most 2^20); block_stride_bytes: bytes from page to page of
- *   kcache / vcache.
+ *   ends inside the prefix keeps its length).  Scores of the rows behind the last kept token in its page become 0.
+ *   row_bytes: bytes of one token's row of one KV head (D * element size, a multiple of 16, at most 2^20);
+ *   block_stride_bytes: bytes from page to page of kcache / vcache.
  *   A destination entry outside [0, num_blocks) drops the rows that it would receive.
  */
 M355_API int m355_kv_evict(void* kcache, void* vcache, float* scores, const int32_t* block_tables, const int32_t* ctx_lens,
